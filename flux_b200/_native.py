@@ -236,27 +236,27 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
 
 
 TORCH_CLASSES_PATH = LIBRARY_PATH.with_name("libfluxb200_torch.so")
-_TORCH_CLASSES: bool | None = None
+torch_classes_loaded = False
 
 
 def load_torch_classes() -> bool:
     """Register ``torch.classes.flux.NativeSmolLM2Decode`` / ``NativeSmolLM2Prefill``
     and the serving operators of ``torch.ops.flux`` (``libfluxb200_torch.so``,
     the reference's custom-class surface and the paged-cache and logits
-    operators over this library); False when that library is not built or does not load.  The C
-    library loads first so both share one copy of it."""
-    global _TORCH_CLASSES
-    if _TORCH_CLASSES is None:
-        _TORCH_CLASSES = False
-        if TORCH_CLASSES_PATH.exists():
-            try:
-                load()
-                import torch
-                torch.classes.load_library(str(TORCH_CLASSES_PATH))
-                _TORCH_CLASSES = True
-            except (OSError, RuntimeError, NativeLibraryUnavailable):
-                _TORCH_CLASSES = False
-    return _TORCH_CLASSES
+    operators over this library); False when that library is not built or does
+    not load, until it does: only success is remembered, so a process may build
+    the library and go on.  The C library loads first so both share one copy of
+    it."""
+    global torch_classes_loaded
+    if not torch_classes_loaded and TORCH_CLASSES_PATH.exists():
+        try:
+            load()
+            import torch
+            torch.classes.load_library(str(TORCH_CLASSES_PATH))
+            torch_classes_loaded = True
+        except (OSError, RuntimeError, NativeLibraryUnavailable):
+            pass
+    return torch_classes_loaded
 
 
 def is_available() -> bool:

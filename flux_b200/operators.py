@@ -905,19 +905,18 @@ def cublaslt_linear_config_out(input, weight, output, workspace, algorithm: Cubl
 
 # ------------------------- paged cache and logits (csrc/torch_operators.cpp)
 
-_SERVING = _native.load_torch_classes()  # registers the schemas; False when the library is not built
+_native.load_torch_classes()  # registers the schemas, if the library is built
 
 
-def _serving_available() -> bool:
-    return _SERVING
+def native_paged_cache_is_available() -> bool:
+    return _native.load_torch_classes()
 
 
-native_paged_cache_is_available = _serving_available
-native_logits_process_is_available = _serving_available
+native_logits_process_is_available = native_paged_cache_is_available
 
 
 def _require_serving(what: str) -> None:
-    if not _SERVING:
+    if not _native.torch_classes_loaded and not _native.load_torch_classes():
         _require_native(what)
         raise RuntimeError(f"Flux native {what} is not built: {_native.TORCH_CLASSES_PATH} is missing or does not load; "
                            "run `python -m flux_b200.build`")
