@@ -7,6 +7,7 @@ point raises :class:`NativeLibraryUnavailable` -- there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import mmap
 import os
 from pathlib import Path
 
@@ -210,6 +211,17 @@ _LIB: ctypes.CDLL | None = None
 _LOAD_ERROR: Exception | None = None
 
 
+def _missing(library: Path, names) -> str | None:
+    """The first of the names that the library's file does not hold, if any.  The
+    file is looked through before it is loaded: a loaded library stays, and
+    would be found again in the place of one rebuilt at the same path."""
+    with open(library, "rb") as file:
+        if os.fstat(file.fileno()).st_size == 0:
+            return next(iter(names))
+        with mmap.mmap(file.fileno(), 0, access=mmap.ACCESS_READ) as data:
+            return next((name for name in names if data.find(name.encode() + b"\0") < 0), None)
+
+
 def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
     """Load (once) and return the library with every signature declared."""
     global _LIB, _LOAD_ERROR
@@ -220,6 +232,11 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
         _LOAD_ERROR = NativeLibraryUnavailable(
             f"flux_b200 native library is not built ({target} is missing); "
             "run `python -m flux_b200.build`")
+        raise _LOAD_ERROR
+    missing = _missing(target, SIGNATURES)
+    if missing is not None:
+        _LOAD_ERROR = NativeLibraryUnavailable(
+            f"{target} is an older build, without {missing}; run `python -m flux_b200.build`")
         raise _LOAD_ERROR
     try:
         lib = ctypes.CDLL(str(target))
@@ -236,6 +253,7 @@ def load(path: str | os.PathLike | None = None) -> ctypes.CDLL:
 
 
 TORCH_CLASSES_PATH = LIBRARY_PATH.with_name("libfluxb200_torch.so")
+TORCH_ENTRIES = ["paged_gqa_decode_attention", "logits_process"]  # operators it has to register
 torch_classes_loaded = False
 
 
@@ -243,14 +261,16 @@ def load_torch_classes() -> bool:
     """Register ``torch.classes.flux.NativeSmolLM2Decode`` / ``NativeSmolLM2Prefill``
     and the serving operators of ``torch.ops.flux`` (``libfluxb200_torch.so``,
     the reference's custom-class surface and the paged-cache and logits
-    operators over this library); False when that library is not built or does
-    not load, until it does: only success is remembered, so a process may build
+    operators over this library); False when that library is not built, older
+    than the package or does not load, until it does: only success is remembered, so a process may build
     the library and go on.  The C library loads first so both share one copy of
     it."""
     global torch_classes_loaded
     if not torch_classes_loaded and TORCH_CLASSES_PATH.exists():
         try:
             load()
+            if _missing(TORCH_CLASSES_PATH, TORCH_ENTRIES) is not None:
+                return False  # an older build
             import torch
             torch.classes.load_library(str(TORCH_CLASSES_PATH))
             torch_classes_loaded = True

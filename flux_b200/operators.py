@@ -918,8 +918,8 @@ native_logits_process_is_available = native_paged_cache_is_available
 def _require_serving(what: str) -> None:
     if not _native.torch_classes_loaded and not _native.load_torch_classes():
         _require_native(what)
-        raise RuntimeError(f"Flux native {what} is not built: {_native.TORCH_CLASSES_PATH} is missing or does not load; "
-                           "run `python -m flux_b200.build`")
+        raise RuntimeError(f"Flux native {what} is not built: {_native.TORCH_CLASSES_PATH} is missing, older than the "
+                           "package or does not load; run `python -m flux_b200.build`")
 
 
 def paged_qkv_rope_cache_native(packed_qkv, cos, sin, key_pages, value_pages, page_table, positions, sequences=None):

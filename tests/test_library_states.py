@@ -1,5 +1,5 @@
 """What a process sees of the native libraries as they come and go: nothing
-built yet, built while the process runs.  Each case runs in a process of its
+built yet, built while the process runs, older than the package.  Each case runs in a process of its
 own on a copy of the package, where building means putting this checkout's
 libraries in place (or compiling, where it has none)."""
 
@@ -93,4 +93,58 @@ def test_operators_are_registered_by_the_import(copy):
 import flux_b200
 torch.ops.flux.paged_gqa_decode_attention
 torch.ops.flux.logits_process
+""")
+
+
+def older(copy):
+    """Libraries from before some entry points were added."""
+    lib = copy / "flux_b200" / "_lib"
+    lib.mkdir()
+    for name, symbol in (("libfluxb200", "fx_last_error"), ("libfluxb200_torch", "flux_torch")):
+        source = copy / f"{name}.c"
+        source.write_text(f'const char* {symbol}(void) {{ return ""; }}\n')
+        subprocess.run(["cc", "-shared", "-fPIC", str(source), "-o", str(lib / f"{name}.so")], check=True)
+
+
+def test_older_libraries_are_refused_and_rebuilt(copy):
+    """The package imports beside libraries that lack entry points, says so, and works once they are rebuilt."""
+    older(copy)
+    run(copy, """
+import flux_b200
+from flux_b200 import _native
+from flux_b200 import operators as ops
+assert not ops.native_paged_cache_is_available() and not flux_b200.is_available()
+assert isinstance(_native.load_error(), _native.NativeLibraryUnavailable)
+refused("older build")
+build()
+refused("CUDA tensors are required")
+assert _native.load_error() is None
+""")
+
+
+def test_older_libraries_are_replaced_by_the_build_alone(copy):
+    older(copy)
+    run(copy, """
+import flux
+build()
+refused("CUDA tensors are required")
+torch.classes.flux.NativeSmolLM2Decode
+""")
+
+
+def test_an_older_torch_library_beside_a_new_one(copy):
+    """As left by a build that ended between the two."""
+    older(copy)
+    run(copy, """
+import flux_b200.build as b
+if built[0].exists():
+    shutil.copy2(built[0], str(b.LIBRARY) + ".new")
+    Path(str(b.LIBRARY) + ".new").replace(b.LIBRARY)
+else:
+    b.build()
+from flux_b200 import operators as ops
+assert ops.native_rmsnorm_is_available() and not ops.native_paged_cache_is_available()
+refused("older")
+build()
+refused("CUDA tensors are required")
 """)
