@@ -7,6 +7,7 @@ point raises :class:`NativeLibraryUnavailable` -- there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import hashlib
 import mmap
 import os
 from pathlib import Path
@@ -277,6 +278,31 @@ def load_torch_classes() -> bool:
         except (OSError, RuntimeError, NativeLibraryUnavailable):
             pass
     return torch_classes_loaded
+
+
+# Written by the build: the digest of the sources that the libraries were built from.
+SOURCES_PATH = LIBRARY_PATH.with_name("sources.sha256")
+
+
+def sources_digest() -> str:
+    package = LIBRARY_PATH.parents[1]
+    files = [*package.glob("csrc/*"), *package.parent.glob("include/*.h")]
+    h = hashlib.sha256()
+    for path in sorted(p for p in files if p.suffix in (".cu", ".cuh", ".cpp", ".h")):
+        h.update(f"{path.name} {path.stat().st_size}\n".encode())
+        h.update(path.read_bytes())
+    return h.hexdigest()
+
+
+def load_current_torch_classes() -> bool:
+    """:func:`load_torch_classes` for the import of the package, where no one
+    has asked for the library yet: one built from other sources is left alone,
+    since a process that goes on to rebuild it could not load the new one."""
+    try:
+        current = SOURCES_PATH.read_text() == sources_digest()
+    except OSError:
+        return False
+    return current and load_torch_classes()
 
 
 def is_available() -> bool:

@@ -23,6 +23,8 @@ import sys
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
+from flux_b200 import _native
+
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
@@ -112,8 +114,15 @@ def _torch_flags() -> tuple[list[str], list[str]]:
 
 def build_torch_classes(verbose: bool = False) -> Path:
     """The library of the ``torch.classes.flux`` classes and the serving
-    operators (links ``libfluxb200.so`` and libtorch)."""
-    library = build(verbose=verbose)
+    operators (links ``libfluxb200.so`` and libtorch), and the record of the
+    sources that both were built from."""
+    digest = _native.sources_digest()
+    _build_torch_library(build(verbose=verbose), verbose)
+    _native.SOURCES_PATH.write_text(digest)
+    return TORCH_LIBRARY
+
+
+def _build_torch_library(library: Path, verbose: bool) -> None:
     flags, link = _torch_flags()
     stamp = BUILD / "torch_classes.stamp"
     h = hashlib.sha256()
@@ -123,7 +132,7 @@ def build_torch_classes(verbose: bool = False) -> Path:
     digest = h.hexdigest()
     if (TORCH_LIBRARY.exists() and stamp.exists() and stamp.read_text() == digest
             and TORCH_LIBRARY.stat().st_mtime >= library.stat().st_mtime):
-        return TORCH_LIBRARY
+        return
     compiler = os.environ.get("CXX", "g++")
 
     def run(cmd: list[str]) -> None:
@@ -142,7 +151,6 @@ def build_torch_classes(verbose: bool = False) -> Path:
          "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda"])
     os.replace(tmp, TORCH_LIBRARY)
     stamp.write_text(digest)
-    return TORCH_LIBRARY
 
 
 def main(argv: list[str] | None = None) -> int:

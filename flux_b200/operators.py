@@ -905,7 +905,7 @@ def cublaslt_linear_config_out(input, weight, output, workspace, algorithm: Cubl
 
 # ------------------------- paged cache and logits (csrc/torch_operators.cpp)
 
-_native.load_torch_classes()  # registers the schemas, if the library is built
+_native.load_current_torch_classes()  # registers the schemas; otherwise the first call does
 
 
 def native_paged_cache_is_available() -> bool:

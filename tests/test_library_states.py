@@ -1,7 +1,8 @@
 """What a process sees of the native libraries as they come and go: nothing
-built yet, built while the process runs, older than the package.  Each case runs in a process of its
-own on a copy of the package, where building means putting this checkout's
-libraries in place (or compiling, where it has none)."""
+built yet, built while the process runs, older than the package, built from
+other sources.  Each case runs in a process of its own on a copy of the package,
+where building means putting this checkout's libraries in place (or compiling,
+where it has none)."""
 
 from __future__ import annotations
 
@@ -33,6 +34,7 @@ def build():
             for p in built:
                 shutil.copy2(p, b.LIB_DIR / (p.name + ".new"))
                 (b.LIB_DIR / (p.name + ".new")).replace(b.LIB_DIR / p.name)
+            b._native.SOURCES_PATH.write_text(b._native.sources_digest())
             return b.TORCH_LIBRARY
         b.build_torch_classes = place
     g.build("no reference checkout")
@@ -147,4 +149,26 @@ assert ops.native_rmsnorm_is_available() and not ops.native_paged_cache_is_avail
 refused("older")
 build()
 refused("CUDA tensors are required")
+""")
+
+
+def test_a_build_from_other_sources_is_not_loaded_by_the_import(copy):
+    """Complete libraries of sources that have changed since: the rebuild's code is what the process goes on with."""
+    run(copy, "build()")
+    source = copy / "flux_b200" / "csrc" / "logits.cu"
+    source.write_text(source.read_text() + "\n")
+    run(copy, """
+import flux_b200, os
+from flux_b200 import _native
+old = os.stat(_native.LIBRARY_PATH).st_ino
+assert not _native.torch_classes_loaded
+build()
+mapped = [line.split() for line in open("/proc/self/maps") if line.rstrip().endswith("libfluxb200.so")]
+assert mapped and {int(fields[4]) for fields in mapped} == {os.stat(_native.LIBRARY_PATH).st_ino} != {old}
+refused("CUDA tensors are required")
+""")
+    run(copy, """
+import flux_b200
+from flux_b200 import _native
+assert _native.torch_classes_loaded  # the record follows the build
 """)
