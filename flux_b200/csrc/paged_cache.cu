@@ -249,9 +249,10 @@ fx_status launch_write(const WriteArgs& a, cudaStream_t stream) {
     const auto aligned = [](const void* p, int64_t stride_bytes) {
         return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride_bytes % 16 == 0;
     };
-    const bool pieces = a.dim / 2 % N == 0 && aligned(a.packed, a.packed_stride * sizeof(T)) &&
+    const bool pieces = a.dim / 2 % N == 0 && a.dim / 2 >= N && aligned(a.packed, a.packed_stride * sizeof(T)) &&
                         aligned(a.cos, a.cos_stride * sizeof(float)) && aligned(a.sin, a.sin_stride * sizeof(float)) &&
                         aligned(a.query, 0);
+    if (!pieces) return launch_write_pieces<T, P, 1, 1>(a, 1, stream);
     const int64_t heads = a.query_heads + 2 * a.kv_heads;
     // Heads of a thread: as few groups of them as still give every SM its four CTAs,
     // so that all threads are there at once; one head each where that leaves fewer
@@ -259,7 +260,6 @@ fx_status launch_write(const WriteArgs& a, cudaStream_t stream) {
     // with 16, 63 with one; 1024 tokens 8.3, 10.3 with one).
     const int64_t groups = std::max<int64_t>(1, 148 * 4 * kWriteThreads / (a.tokens * (a.dim / 2 / N)));
     const int64_t span = (heads + groups - 1) / groups;
-    if (!pieces) return launch_write_pieces<T, P, 1, 1>(a, 1, stream);
     if (span >= 4) return launch_write_pieces<T, P, N, 4>(a, static_cast<int>((span + 3) / 4 * 4), stream);
     return launch_write_pieces<T, P, N, 1>(a, 1, stream);
 }
