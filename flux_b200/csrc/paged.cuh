@@ -47,10 +47,10 @@ struct FastDivide {
         while ((int64_t{1} << s) < d) ++s;
         return {static_cast<uint32_t>(d), static_cast<uint32_t>(((uint64_t{1} << (31 + s)) + d - 1) / d), 31 + s};
     }
-    __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
+    __host__ __device__ __forceinline__ uint32_t quotient(uint32_t n) const {
         return static_cast<uint32_t>((static_cast<uint64_t>(n) * magic) >> shift);
     }
-    __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t* remainder) const {
+    __host__ __device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t* remainder) const {
         const uint32_t q = quotient(n);
         *remainder = n - q * divisor;
         return q;

@@ -64,14 +64,23 @@ __device__ __forceinline__ float* paged_pieces(const PagedAttend& a) {
     return a.workspace + kPagedMaxGrid * kPagedDescriptor + 2 * kPagedUnits;
 }
 
-__device__ __forceinline__ int paged_rows(const PagedAttend& a, int b) {
+__host__ __device__ __forceinline__ int paged_rows(const PagedAttend& a, int b) {
     const int64_t n = a.lengths[b];
     return n < 0 ? 0 : (n > a.capacity ? a.capacity : static_cast<int>(n));
 }
 
 template <int kTile>
-__device__ __forceinline__ int paged_tiles(int rows) {
-    return rows <= kTile ? 1 : (rows + kTile - 1) / kTile;
+__host__ __device__ __forceinline__ int paged_tiles(int rows) {
+    return rows <= kTile ? 1 : (rows - 1) / kTile + 1;  // for up to 2^31 - 1 rows
+}
+
+// The first of `total` tiles that CTA i of `ctas` takes.
+__host__ __device__ __forceinline__ int paged_first(int64_t i, int total, int ctas) {
+    return static_cast<int>(i * total / ctas);
+}
+// The CTA that takes tile t.
+__host__ __device__ __forceinline__ int paged_owner(int64_t t, int total, int ctas) {
+    return static_cast<int>(((t + 1) * ctas - 1) / total);
 }
 
 // Where a CTA starts: tile `tile` of KV head `head` of sequence `b`, and how
@@ -81,6 +90,17 @@ struct PagedStart {
     int rows;         // of sequence b
     int total, ctas;  // tiles of all units, CTAs that have any
 };
+
+// Sequence, KV head and tile of the tile `rest` from the start of sequence b on.
+template <int kTile>
+__host__ __device__ __forceinline__ PagedStart paged_locate(const PagedAttend& a, int b, int rest) {
+    for (; b < a.batch; ++b) {
+        const int rows = paged_rows(a, b), tiles = paged_tiles<kTile>(rows);
+        if (rest < tiles * a.kv_heads) return {b, rest / tiles, rest % tiles, 0, rows, 0, 0};
+        rest -= tiles * a.kv_heads;
+    }
+    return {};
+}
 
 // Each thread sums the tiles of a run of sequences, the CTA scans the sums, and
 // the thread whose run holds the CTA's first tile looks it up.
@@ -129,19 +149,14 @@ __device__ __forceinline__ void paged_start(const PagedAttend& a, PagedStart* st
     }
     total *= a.kv_heads;
     const int ctas = min(static_cast<int>(gridDim.x), total);
-    const int first = static_cast<int>(static_cast<int64_t>(blockIdx.x) * total / ctas);
-    const int last = static_cast<int>((static_cast<int64_t>(blockIdx.x) + 1) * total / ctas);
+    const int first = paged_first(blockIdx.x, total, ctas), last = paged_first(blockIdx.x + int64_t{1}, total, ctas);
     if (tid == 0 && static_cast<int>(blockIdx.x) >= ctas) *start = {0, 0, 0, 0, 0, total, ctas};
     if (static_cast<int>(blockIdx.x) < ctas && before * a.kv_heads <= first && first < (before + sum) * a.kv_heads) {
-        int b = b0, rest = first - before * a.kv_heads;
-        for (; b < b1; ++b) {
-            const int rows = paged_rows(a, b), tiles = paged_tiles<kTile>(rows);
-            if (rest < tiles * a.kv_heads) {
-                *start = {b, rest / tiles, rest % tiles, last - first, rows, total, ctas};
-                break;
-            }
-            rest -= tiles * a.kv_heads;
-        }
+        PagedStart found = paged_locate<kTile>(a, b0, first - before * a.kv_heads);
+        found.left = last - first;
+        found.total = total;
+        found.ctas = ctas;
+        *start = found;
     }
     __syncthreads();
 }
@@ -151,7 +166,7 @@ template <int kTile>
 struct PagedCursor {
     int b, head, tile, left, rows, tiles;
 
-    __device__ __forceinline__ void begin(const PagedStart& s) {
+    __host__ __device__ __forceinline__ void begin(const PagedStart& s) {
         b = s.b;
         head = s.head;
         tile = s.tile;
@@ -160,14 +175,14 @@ struct PagedCursor {
         tiles = paged_tiles<kTile>(rows);
     }
     // Tiles of the current unit that belong to this CTA, from the current one on.
-    __device__ __forceinline__ int piece() const { return min(tiles - tile, left); }
-    __device__ __forceinline__ void next(const PagedAttend& a) {
+    __host__ __device__ __forceinline__ int piece() const { return tiles - tile < left ? tiles - tile : left; }
+    __host__ __device__ __forceinline__ void next(const PagedAttend& a) {
         --left;
         if (++tile < tiles || left == 0) return;
         tile = 0;
         if (++head == a.kv_heads) {
             head = 0;
-            b = min(b + 1, a.batch - 1);
+            b = b + 1 < a.batch ? b + 1 : a.batch - 1;
             rows = paged_rows(a, b);
             tiles = paged_tiles<kTile>(rows);
         }
@@ -175,9 +190,15 @@ struct PagedCursor {
 };
 
 struct PagedRow {
-    int page, head, row;
-    int rows;  // of the sequence from `row` on
-    bool any;  // a tile is left (the same for all lanes)
+    int page, head;
+    uint32_t row;  // of the last tile of 2^31 - 1 rows, some are numbered beyond them
+    int rows;      // of the sequence from `row` on
+    bool any;      // a tile is left (the same for all lanes)
+
+    __host__ __device__ __forceinline__ static PagedRow at(int head, int tile_row, int offset, int rows, bool any) {
+        const uint32_t row = static_cast<uint32_t>(tile_row) + static_cast<uint32_t>(offset);
+        return {-1, head, row, static_cast<int>(static_cast<uint32_t>(rows) - row), any};
+    }
 };
 
 // How the 16-byte pieces of a row are exchanged in shared memory, so that the
@@ -207,11 +228,10 @@ struct PagedRing {
     template <int kTile>
     static __device__ __forceinline__ PagedRow look(const PagedAttend& a, PagedCursor<kTile>& at) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        const int mine = runs(a) ? 0 : lane, row = at.tile * kTile + warp * R + mine;
-        PagedRow r{-1, at.head, row, at.rows - row, at.left > 0};
+        const int mine = runs(a) ? 0 : lane;
+        PagedRow r = PagedRow::at(at.head, at.tile * kTile, warp * R + mine, at.rows, at.left > 0);
         if (!r.any) return r;
-        if (mine < R && r.rows > 0)
-            r.page = __ldg(a.table + at.b * a.table_stride + a.page_size.quotient(static_cast<uint32_t>(row)));
+        if (mine < R && r.rows > 0) r.page = __ldg(a.table + at.b * a.table_stride + a.page_size.quotient(r.row));
         at.next(a);
         return r;
     }
@@ -220,8 +240,8 @@ struct PagedRing {
         constexpr int kSteps = (R * kChunks + 31) / 32, kElements = 16 / static_cast<int>(sizeof(P));
         const int lane = threadIdx.x & 31;
         if (!at.any) return;
-        uint32_t slot;
-        a.page_size.quotient(static_cast<uint32_t>(at.row), &slot);
+        uint32_t slot = 0;
+        if (at.page >= 0) a.page_size.quotient(at.row, &slot);  // a row with a page is below 2^31
         const uint32_t head = a.share.quotient(static_cast<uint32_t>(at.head));
         const P* keys = static_cast<const P*>(a.keys);
         const P* values = static_cast<const P*>(a.values);
@@ -373,8 +393,8 @@ __device__ __forceinline__ void paged_join(const PagedAttend& a, const PagedStar
     if (threadIdx.x == 0 && (last || first == 0)) {
         // For the merge kernel: the unit that starts in this CTA and ends in another.
         const bool open = first == 0 && !whole;
-        const int64_t end = (static_cast<int64_t>(blockIdx.x) + 1) * start.total / start.ctas + (tiles - count) - 1;
-        const int to = open ? static_cast<int>(((end + 1) * start.ctas - 1) / start.total) : -1;
+        const int64_t end = int64_t{paged_first(blockIdx.x + int64_t{1}, start.total, start.ctas)} + (tiles - count) - 1;
+        const int to = open ? paged_owner(end, start.total, start.ctas) : -1;
         int* note = reinterpret_cast<int*>(a.workspace) + blockIdx.x * kPagedDescriptor;
         if (last) {
             note[0] = b;
@@ -425,7 +445,7 @@ inline bool paged_whole(const PagedAttend& a, int sms) {
 template <int kTile>
 inline int paged_grid(const PagedAttend& a, int sms, int per_sm) {
     const int64_t most =
-        static_cast<int64_t>(a.batch) * a.kv_heads * (a.whole ? 1 : (a.capacity + kTile - 1) / kTile);
+        static_cast<int64_t>(a.batch) * a.kv_heads * (a.whole ? 1 : paged_tiles<kTile>(a.capacity));
     int64_t grid = static_cast<int64_t>(sms) * per_sm;
     if (grid > kPagedMaxGrid) grid = kPagedMaxGrid;
     return static_cast<int>(grid < most ? grid : most);
