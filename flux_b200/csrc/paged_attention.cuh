@@ -71,7 +71,7 @@ __host__ __device__ __forceinline__ int paged_rows(const PagedAttend& a, int b) 
 
 template <int kTile>
 __host__ __device__ __forceinline__ int paged_tiles(int rows) {
-    return rows <= kTile ? 1 : (rows - 1) / kTile + 1;  // for up to 2^31 - 1 rows
+    return rows <= kTile ? 1 : static_cast<int>((static_cast<uint32_t>(rows) + (kTile - 1)) / kTile);
 }
 
 // The first of `total` tiles that CTA i of `ctas` takes.
@@ -175,14 +175,14 @@ struct PagedCursor {
         tiles = paged_tiles<kTile>(rows);
     }
     // Tiles of the current unit that belong to this CTA, from the current one on.
-    __host__ __device__ __forceinline__ int piece() const { return tiles - tile < left ? tiles - tile : left; }
+    __host__ __device__ __forceinline__ int piece() const { return min(tiles - tile, left); }
     __host__ __device__ __forceinline__ void next(const PagedAttend& a) {
         --left;
         if (++tile < tiles || left == 0) return;
         tile = 0;
         if (++head == a.kv_heads) {
             head = 0;
-            b = b + 1 < a.batch ? b + 1 : a.batch - 1;
+            b = min(b + 1, a.batch - 1);
             rows = paged_rows(a, b);
             tiles = paged_tiles<kTile>(rows);
         }
@@ -240,8 +240,8 @@ struct PagedRing {
         constexpr int kSteps = (R * kChunks + 31) / 32, kElements = 16 / static_cast<int>(sizeof(P));
         const int lane = threadIdx.x & 31;
         if (!at.any) return;
-        uint32_t slot = 0;
-        if (at.page >= 0) a.page_size.quotient(at.row, &slot);  // a row with a page is below 2^31
+        uint32_t slot;
+        a.page_size.quotient(at.row & 0x7fffffffu, &slot);  // a row with a page is below 2^31
         const uint32_t head = a.share.quotient(static_cast<uint32_t>(at.head));
         const P* keys = static_cast<const P*>(a.keys);
         const P* values = static_cast<const P*>(a.values);
