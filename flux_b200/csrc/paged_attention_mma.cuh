@@ -51,8 +51,15 @@ struct Mma<__nv_bfloat16> {
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
     // The nearest 16-bit values of x and y, and what they leave in x and y.
-    static __device__ __forceinline__ uint32_t term(float& x, float& y) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    static __device__ __forceinline__ uint32_t term(float& x, float& y) { return term(x, y, x, y); }
+    // The first of several: bfloat16 ends half a place before FP32 does, and
+    // there the largest one is taken.
+    static __device__ __forceinline__ uint32_t first_term(float& x, float& y) {
+        const float most = __uint_as_float(0x7f7f0000u);
+        return term(x, y, fminf(fmaxf(x, -most), most), fminf(fmaxf(y, -most), most));
+    }
+    static __device__ __forceinline__ uint32_t term(float& x, float& y, float near_x, float near_y) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(near_x, near_y);
         const float2 f = __bfloat1622float2(h);
         x -= f.x;
         y -= f.y;
@@ -75,6 +82,7 @@ struct Mma<__half> {
         y -= f.y;
         return *reinterpret_cast<const uint32_t*>(&h);
     }
+    static __device__ __forceinline__ uint32_t first_term(float& x, float& y) { return term(x, y); }  // scaled queries
     static constexpr float kWeightBits = 14.0f;
 };
 
@@ -200,7 +208,7 @@ __global__ void __launch_bounds__(MmaShape<T, Q, DP, Heads>::kThreads, MmaShape<
 #pragma unroll
                 for (int across = 0; across < 2; ++across) {
                     float x = element(i, 0, across, 0) * factor[0], y = element(i, 0, across, 1) * factor[0];
-                    w[0][2 * across] = Mma<T>::term(x, y);
+                    w[0][2 * across] = S::kExact ? Mma<T>::first_term(x, y) : Mma<T>::term(x, y);
                     if constexpr (S::kExact) {
                         const uint32_t two = Mma<T>::term(x, y), three = Mma<T>::term(x, y);
                         if constexpr (kQuarters) {
@@ -222,10 +230,13 @@ __global__ void __launch_bounds__(MmaShape<T, Q, DP, Heads>::kThreads, MmaShape<
 #pragma unroll
                     for (int e = 0; e < 2; ++e) x[r][e] = element(i, r & 1, r >> 1, e) * factor[r & 1];
 #pragma unroll
-                for (int term = 0; term < S::kQueryOperands; ++term)
-                    queries[(term * kSteps + i) * 32 + lane] =
-                        make_uint4(Mma<T>::term(x[0][0], x[0][1]), Mma<T>::term(x[1][0], x[1][1]),
-                                   Mma<T>::term(x[2][0], x[2][1]), Mma<T>::term(x[3][0], x[3][1]));
+                for (int term = 0; term < S::kQueryOperands; ++term) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        w[r] = S::kExact && term == 0 ? Mma<T>::first_term(x[r][0], x[r][1]) : Mma<T>::term(x[r][0], x[r][1]);
+                    queries[(term * kSteps + i) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             }
         }
         __syncthreads();

@@ -36,8 +36,17 @@ struct KeyPieces { static __device__ __forceinline__ int at(int piece, int row) 
 struct ValuePieces { static __device__ __forceinline__ int at(int piece, int row) { return piece ^ (((row >> 1) & 3) << 1); } };
 
 // hi: x to the nearest TF32 value, ties away from zero (half of its last place
-// is added, the rest cut off); lo: what that leaves, cut off to TF32.
+// is added, the rest cut off); lo: what that leaves, cut off to TF32.  Half a
+// place below the end of FP32's range the nearest value would be infinite: hi
+// is then the largest one, and lo holds more (of an infinity, all).
 __device__ __forceinline__ void split(float x, uint32_t& hi, uint32_t& lo) {
+    float near;  // the smaller magnitude, with x's sign
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(near) : "f"(x), "f"(__uint_as_float(0x7f7fefffu)));
+    hi = (__float_as_uint(near) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+// The same of a weight, which is at most 1.
+__device__ __forceinline__ void split_weight(float x, uint32_t& hi, uint32_t& lo) {
     hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
@@ -197,13 +206,13 @@ __global__ void __launch_bounds__(Tf32Shape<DP, Heads>::kThreads, (Tf32Shape<DP,
             // Rows k = c and c + 4 of the second product are keys 2 c and 2 c + 1.
             uint32_t ph[4], pl[4];
             if constexpr (S::kPacked) {
-                split(s[0], ph[0], ph[1]);
-                split(s[1], ph[2], ph[3]);
+                split_weight(s[0], ph[0], ph[1]);
+                split_weight(s[1], ph[2], ph[3]);
             } else {
-                split(s[0], ph[0], pl[0]);
-                split(s[2], ph[1], pl[1]);
-                split(s[1], ph[2], pl[2]);
-                split(s[3], ph[3], pl[3]);
+                split_weight(s[0], ph[0], pl[0]);
+                split_weight(s[2], ph[1], pl[1]);
+                split_weight(s[1], ph[2], pl[2]);
+                split_weight(s[3], ph[3], pl[3]);
             }
 #pragma unroll
             for (int j = 0; j < DP / 8; j += 4) {  // 32 dims: columns g of four products are dims 4 g, 4 g + 1, ...

@@ -37,3 +37,51 @@ def test_attention_over_the_longest_table(page, query, pages, group):
     lengths.fill_(columns * page - 1)  # without the last row
     out = ops.paged_gqa_decode_attention_native(q.cuda(), kc, vc, table, lengths, 0.25)
     _assert_attention(out, q, k, v, short, torch.tensor([4 * page - 1]), 0.25)
+
+
+TOP = torch.finfo(torch.float32).max
+
+
+@pytest.mark.parametrize("dim", [16, 64, 128, 256])
+@pytest.mark.parametrize("group", [1, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("where", ["values", "keys", "queries"])
+def test_attention_with_the_largest_finite_values(group, dim, where):
+    """Elements up to the largest float32, among them those that round up to infinity in fewer bits, beside operands
+    so small that every product and sum stays in range."""
+    case = [_randn((40, 2, 16, dim), torch.float32, 1), _randn((40, 2, 16, dim), torch.float32, 2),
+            _randn((2, 2 * group, 1, dim), torch.float32, 3)]
+    k, v, q = case
+    lengths, scale = torch.tensor([1, 300]), 0.25
+    table = ref.table_for([1, 300], 16, 40)
+    near = torch.tensor([TOP, -TOP, TOP * (1 - 2.0 ** -13), TOP * (1 - 2.0 ** -10), -TOP * (1 - 2.0 ** -12), TOP * 0.999])
+    if where == "values":
+        v *= 2.0 ** 10
+        first = int(table[0, 0])
+        v[first, :, 0, :6], v[first, :, 0, -1] = near, -TOP  # all the weight: the output is the value
+        p = int(table[1, 3])
+        v[p, :, 5, 3:9] = near
+        k[p, :, 5] = 0  # about the mean weight, far below 1
+    elif where == "keys":
+        k *= 2.0 ** 100
+        q *= 2.0 ** -100
+        for b in range(2):
+            k[int(table[b, 0]), :, 0, :6] = near
+        q[..., :6] = q[..., :6].sign() * 2.0 ** -126
+    else:
+        q[..., :6] = near * (1 + torch.arange(2 * group).view(1, -1, 1, 1) % 2 * -2.0 ** -11)
+        k[..., :6] = k[..., :6].sign() * 2.0 ** -126
+    assert all(t.isfinite().all() for t in (k, v, q))
+    out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lengths.cuda(), scale)
+    _assert_attention(out, q, k, v, table, lengths, scale)
+
+
+@pytest.mark.parametrize("group", [1, 3, 4, 5, 8, 9, 16])
+def test_attention_with_the_largest_queries_on_16_bit_pages(group):
+    """Float32 queries up to the largest, where bfloat16 ends earlier."""
+    k, v = (_randn((40, 2, 16, 64), torch.bfloat16, seed) for seed in (1, 2))
+    q = _randn((2, 2 * group, 1, 64), torch.float32, 3)
+    table, lengths = ref.table_for([1, 300], 16, 40), torch.tensor([1, 300])
+    q[..., :4] = torch.tensor([TOP, -TOP, TOP * (1 - 2.0 ** -9), -TOP * (1 - 2.0 ** -10)])
+    k[..., :4] = k[..., :4].sign() * 2.0 ** -126
+    out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lengths.cuda(), 0.25)
+    _assert_attention(out, q, k, v, table, lengths, 0.25)
