@@ -231,7 +231,7 @@ struct PagedRing {
         const int mine = runs(a) ? 0 : lane;
         PagedRow r = PagedRow::at(at.head, at.tile * kTile, warp * R + mine, at.rows, at.left > 0);
         if (!r.any) return r;
-        if (mine < R && r.rows > 0) r.page = __ldg(a.table + at.b * a.table_stride + a.page_size.quotient(r.row));
+        if (mine < R && r.rows > 0) r.page = a.table[at.b * a.table_stride + a.page_size.quotient(r.row)];
         at.next(a);
         return r;
     }

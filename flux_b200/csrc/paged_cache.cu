@@ -391,13 +391,13 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
         };
 #pragma unroll 4
         for (int64_t i = threadIdx.x; i < count; i += kCopyThreads) {
-            const int64_t s = __ldg(source + i), d = __ldg(destination + i);
+            const int64_t s = source[i], d = destination[i];
             if (moved(s, d)) conflict |= (atomicOr(&written[d >> 5], 1u << (d & 31)) >> (d & 31)) & 1u;
         }
         __syncthreads();
 #pragma unroll 4
         for (int64_t i = threadIdx.x; i < count; i += kCopyThreads) {
-            const int64_t s = __ldg(source + i), d = __ldg(destination + i);
+            const int64_t s = source[i], d = destination[i];
             if (moved(s, d)) conflict |= (written[s >> 5] >> (s & 31)) & 1u;
         }
         conflict = __syncthreads_or(conflict);
