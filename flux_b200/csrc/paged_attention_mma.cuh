@@ -22,10 +22,12 @@
 //
 // float16's narrow range is met by scaling: a query row so that its largest
 // element lies in [2^13, 2^14), the weights by 2^14 (their sum too, so that it
-// cancels).  For FP32 queries P V is added to O with an FP32 instruction: the
-// tensor cores truncate when they accumulate, which over a long sequence would
-// show (2^-25 a step on average, 1000 steps for 16384 rows, far below a 16-bit
-// output's rounding).
+// cancels).  The tensor cores truncate when they accumulate, by 2^-25 a product on
+// average and always towards zero.  For FP32 queries P V is therefore added to O
+// with an FP32 instruction.  For 16-bit queries O is the accumulator, which stays
+// below a 16-bit output's rounding for tables of up to 65536 rows; in longer ones
+// it is summed in runs of 256 tiles, which are joined in FP32 (one run of 4 M rows
+// would be off by 0.8 %).
 //
 // A decode step has one row per head, so the larger tcgen05 tiles (64 or 128
 // rows) would be 4-8 times emptier still and would add a trip through TMEM
@@ -129,12 +131,14 @@ struct MmaShape {
     static_assert(kStages >= 2, "two stages at least");
 };
 
-template <typename T, typename Q, int DP, int Heads>
+// Runs: O is summed in runs of kRun tiles.
+template <typename T, typename Q, int DP, int Heads, bool Runs>
 __global__ void __launch_bounds__(MmaShape<T, Q, DP, Heads>::kThreads, MmaShape<T, Q, DP, Heads>::kPerSm)
     paged_mma_kernel(const __grid_constant__ PagedAttend a) {
     using S = MmaShape<T, Q, DP, Heads>;
     using Ring = typename S::Ring;
     constexpr int kSteps = DP / 16;
+    constexpr int kRun = 256;
     constexpr bool kQuarters = Heads == 4;  // terms in rows 0-3, 4-7 and 8-11
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ PagedStart start;
@@ -234,7 +238,8 @@ __global__ void __launch_bounds__(MmaShape<T, Q, DP, Heads>::kThreads, MmaShape<
                     uint32_t w[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
-                        w[r] = S::kExact && term == 0 ? Mma<T>::first_term(x[r][0], x[r][1]) : Mma<T>::term(x[r][0], x[r][1]);
+                        w[r] = S::kExact && term == 0 ? Mma<T>::first_term(x[r][0], x[r][1])
+                                                      : Mma<T>::term(x[r][0], x[r][1]);
                     queries[(term * kSteps + i) * 32 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
@@ -252,192 +257,237 @@ __global__ void __launch_bounds__(MmaShape<T, Q, DP, Heads>::kThreads, MmaShape<
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) operand(q[i], 0, i);
         }
-        float m[S::kHalves], l[S::kHalves];
-#pragma unroll
-        for (int r = 0; r < S::kHalves; ++r) {
-            m[r] = -INFINITY;
-            l[r] = 0.0f;
-        }
-        float o[DP / 8][4];
-#pragma unroll
-        for (int j = 0; j < DP / 8; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
-
-        for (int t = 0; t < count; ++t) {
-            // Kernels that HBM bounds keep their warps to one tile: apart, they read a
-            // page's rows at different times (64 x 8192 rows of 3 KV heads of 64 16-bit
-            // dims: FP32 queries 72 us, 69 together; 16-bit ones 72 and 68).  With more
-            // products the wait costs more than it gives (92 us, 96).
-            if (S::kWeightOperands == 1) __syncthreads();
-            stream.advance();
-            const uint32_t keys = static_cast<uint32_t>(__cvta_generic_to_shared(stream.keys()));
-            const uint32_t values = keys + Ring::kHalf * 2;
-            float s[2][4] = {}, rest[2][4] = {};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                uint32_t k[4];
-                load_matrices(k, keys + k_row * S::kRowBytes + (((2 * i + k_piece) ^ (k_row & 7)) << 4));
-                if constexpr (!S::kHoldQueries) operand(q[0], 0, i);
-                Mma<T>::run(s[0], q[S::kHoldQueries ? i : 0], k[0], k[1]);
-                Mma<T>::run(s[1], q[S::kHoldQueries ? i : 0], k[2], k[3]);
-#pragma unroll
-                for (int term = 1; term < S::kQueryOperands; ++term) {
-                    operand(q[0], term, i);
-                    Mma<T>::run(rest[0], q[0], k[0], k[1]);
-                    Mma<T>::run(rest[1], q[0], k[2], k[3]);
-                }
-            }
-            if constexpr (S::kExact) {
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2 * S::kHalves; ++e) {
-                        if constexpr (S::kPacked) s[n][e] += s[n][2 + e] + rest[n][e];
-                        else s[n][e] += rest[n][e];
-                        // Both lanes of a head come to the same sum.
-                        if constexpr (kQuarters) s[n][e] += __shfl_xor_sync(0xffffffffu, s[n][e], 16);
-                    }
-            }
-            const uint32_t mask = stream.mask() >> pair;
-            float keep[S::kHalves];
+        float m[S::kHalves], l[S::kHalves], o[DP / 8][4];
+        const auto clear = [&] {
 #pragma unroll
             for (int r = 0; r < S::kHalves; ++r) {
-                float top = m[r];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = s[n][2 * r + e];
-                        x = (mask >> (8 * n + e)) & 1u ? x * scale[r] : -INFINITY;
-                        top = fmaxf(top, x);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float base = top == -INFINITY ? 0.0f : top;
-                keep[r] = exp2f(m[r] - base);
-                m[r] = top;
-                l[r] *= keep[r];
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& x = s[n][2 * r + e];
-                        x = exp2f(x - base + Mma<T>::kWeightBits);
-                        l[r] += x;
-                    }
-            }
-            uint32_t p[S::kWeightOperands][4] = {};
-#pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                if constexpr (S::kPacked) {
-                    const uint32_t one = Mma<T>::term(s[n][0], s[n][1]), two = Mma<T>::term(s[n][0], s[n][1]);
-                    p[0][2 * n] = one;
-                    p[0][2 * n + 1] = two;
-                    if constexpr (S::kExact) {
-                        const uint32_t three = Mma<T>::term(s[n][0], s[n][1]);
-                        if constexpr (kQuarters) {
-                            p[0][2 * n] = leads ? one : two;
-                            p[0][2 * n + 1] = leads ? three : 0u;
-                        } else {
-                            p[S::kWeightOperands - 1][2 * n] = three;
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int term = 0; term < S::kWeightOperands; ++term)
-#pragma unroll
-                        for (int r = 0; r < 2; ++r)
-                            p[term][2 * n + r] = Mma<T>::term(s[n][2 * r], s[n][2 * r + 1]);
-                }
-            }
-            const auto kept = [&](int e) { return keep[S::kHalves == 2 ? e >> 1 : 0]; };
-            if constexpr (!S::kExact) {
-                if (__any_sync(0xffffffffu, kept(0) != 1.0f || kept(2) != 1.0f)) {
-#pragma unroll
-                    for (int j = 0; j < DP / 8; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[j][e] *= kept(e);
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < DP / 8; j += 2) {
-                uint32_t v[4];
-                load_matrices_transposed(v, values + v_row * S::kRowBytes + (((j + v_piece) ^ (v_row & 7)) << 4));
-                if constexpr (!S::kExact) {
-#pragma unroll
-                    for (int term = S::kWeightOperands - 1; term >= 0; --term) {
-                        Mma<T>::run(o[j], p[term], v[0], v[1]);
-                        Mma<T>::run(o[j + 1], p[term], v[2], v[3]);
-                    }
-                    continue;
-                }
-                float x[2][4] = {};
-#pragma unroll
-                for (int term = S::kWeightOperands - 1; term >= 0; --term) {
-                    Mma<T>::run(x[0], p[term], v[0], v[1]);
-                    Mma<T>::run(x[1], p[term], v[2], v[3]);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o[j][e] = fmaf(o[j][e], kept(e), x[0][e]);
-                    o[j + 1][e] = fmaf(o[j + 1][e], kept(e), x[1][e]);
-                }
-            }
-            stream.release();
-        }
-
-        const int width = a.dim + 2;
-        float* mine = states + warp * a.group * width;
-#pragma unroll
-        for (int r = 0; r < S::kHalves; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            const int h = top_head + 8 * r;
-            const bool any = h < a.group && (!kQuarters || leads);
-            if (any && (lane & 3) == 0) {
-                mine[h * width] = m[r];
-                mine[h * width + 1] = l[r];
+                m[r] = -INFINITY;
+                l[r] = 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < DP / 8; ++j)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float x = o[j][2 * r + e];
-                    if constexpr (S::kPacked) x += o[j][2 + e];
-                    if constexpr (kQuarters) x += __shfl_xor_sync(0xffffffffu, x, 16);
-                    if (any && 8 * j < a.dim) mine[h * width + 2 + 8 * j + pair + e] = x;
+                for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
+        };
+        const int width = a.dim + 2;
+        float* mine = states + warp * a.group * width;
+        // Joins the state that the warp left in shared memory to the one it holds.
+        const auto take_back = [&] {
+#pragma unroll
+            for (int r = 0; r < S::kHalves; ++r) {
+                const int h = top_head + 8 * r;
+                const bool any = h < a.group;
+                const float before = any ? mine[h * width] : -INFINITY, sum = any ? mine[h * width + 1] : 0.0f;
+                const float top = fmaxf(m[r], before), base = top == -INFINITY ? 0.0f : top;
+                const float now = exp2f(m[r] - base), then = exp2f(before - base);
+                m[r] = top;
+                l[r] = fmaf(l[r], now, (lane & 3) == 0 ? sum * then : 0.0f);
+#pragma unroll
+                for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float x = any && 8 * j < a.dim ? mine[h * width + 2 + 8 * j + pair + e] : 0.0f;
+                        o[j][2 * r + e] = fmaf(o[j][2 * r + e], now, x * then);
+                        if constexpr (S::kPacked) o[j][2 + e] *= now;
+                    }
+            }
+            __syncwarp();  // all of it is read
+        };
+        int done = 0;
+        do {
+            const int until = Runs ? min(count - done, kRun) : count;
+            clear();
+            for (int t = 0; t < until; ++t) {
+                // Kernels that HBM bounds keep their warps to one tile: apart, they read a
+                // page's rows at different times (64 x 8192 rows of 3 KV heads of 64 16-bit
+                // dims: FP32 queries 72 us, 69 together; 16-bit ones 72 and 68).  With more
+                // products the wait costs more than it gives (92 us, 96).
+                if (S::kWeightOperands == 1) __syncthreads();
+                stream.advance();
+                const uint32_t keys = static_cast<uint32_t>(__cvta_generic_to_shared(stream.keys()));
+                const uint32_t values = keys + Ring::kHalf * 2;
+                float s[2][4] = {}, rest[2][4] = {};
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    uint32_t k[4];
+                    load_matrices(k, keys + k_row * S::kRowBytes + (((2 * i + k_piece) ^ (k_row & 7)) << 4));
+                    if constexpr (!S::kHoldQueries) operand(q[0], 0, i);
+                    Mma<T>::run(s[0], q[S::kHoldQueries ? i : 0], k[0], k[1]);
+                    Mma<T>::run(s[1], q[S::kHoldQueries ? i : 0], k[2], k[3]);
+#pragma unroll
+                    for (int term = 1; term < S::kQueryOperands; ++term) {
+                        operand(q[0], term, i);
+                        Mma<T>::run(rest[0], q[0], k[0], k[1]);
+                        Mma<T>::run(rest[1], q[0], k[2], k[3]);
+                    }
                 }
-        }
+                if constexpr (S::kExact) {
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2 * S::kHalves; ++e) {
+                            if constexpr (S::kPacked) s[n][e] += s[n][2 + e] + rest[n][e];
+                            else s[n][e] += rest[n][e];
+                            // Both lanes of a head come to the same sum.
+                            if constexpr (kQuarters) s[n][e] += __shfl_xor_sync(0xffffffffu, s[n][e], 16);
+                        }
+                }
+                const uint32_t mask = stream.mask() >> pair;
+                float keep[S::kHalves];
+#pragma unroll
+                for (int r = 0; r < S::kHalves; ++r) {
+                    float top = m[r];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& x = s[n][2 * r + e];
+                            x = (mask >> (8 * n + e)) & 1u ? x * scale[r] : -INFINITY;
+                            top = fmaxf(top, x);
+                        }
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    const float base = top == -INFINITY ? 0.0f : top;
+                    keep[r] = exp2f(m[r] - base);
+                    m[r] = top;
+                    l[r] *= keep[r];
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& x = s[n][2 * r + e];
+                            x = exp2f(x - base + Mma<T>::kWeightBits);
+                            l[r] += x;
+                        }
+                }
+                uint32_t p[S::kWeightOperands][4] = {};
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    if constexpr (S::kPacked) {
+                        const uint32_t one = Mma<T>::term(s[n][0], s[n][1]), two = Mma<T>::term(s[n][0], s[n][1]);
+                        p[0][2 * n] = one;
+                        p[0][2 * n + 1] = two;
+                        if constexpr (S::kExact) {
+                            const uint32_t three = Mma<T>::term(s[n][0], s[n][1]);
+                            if constexpr (kQuarters) {
+                                p[0][2 * n] = leads ? one : two;
+                                p[0][2 * n + 1] = leads ? three : 0u;
+                            } else {
+                                p[S::kWeightOperands - 1][2 * n] = three;
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int term = 0; term < S::kWeightOperands; ++term)
+#pragma unroll
+                            for (int r = 0; r < 2; ++r)
+                                p[term][2 * n + r] = Mma<T>::term(s[n][2 * r], s[n][2 * r + 1]);
+                    }
+                }
+                const auto kept = [&](int e) { return keep[S::kHalves == 2 ? e >> 1 : 0]; };
+                if constexpr (!S::kExact) {
+                    if (__any_sync(0xffffffffu, kept(0) != 1.0f || kept(2) != 1.0f)) {
+#pragma unroll
+                        for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[j][e] *= kept(e);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < DP / 8; j += 2) {
+                    uint32_t v[4];
+                    load_matrices_transposed(v, values + v_row * S::kRowBytes + (((j + v_piece) ^ (v_row & 7)) << 4));
+                    if constexpr (!S::kExact) {
+#pragma unroll
+                        for (int term = S::kWeightOperands - 1; term >= 0; --term) {
+                            Mma<T>::run(o[j], p[term], v[0], v[1]);
+                            Mma<T>::run(o[j + 1], p[term], v[2], v[3]);
+                        }
+                        continue;
+                    }
+                    float x[2][4] = {};
+#pragma unroll
+                    for (int term = S::kWeightOperands - 1; term >= 0; --term) {
+                        Mma<T>::run(x[0], p[term], v[0], v[1]);
+                        Mma<T>::run(x[1], p[term], v[2], v[3]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        o[j][e] = fmaf(o[j][e], kept(e), x[0][e]);
+                        o[j + 1][e] = fmaf(o[j + 1][e], kept(e), x[1][e]);
+                    }
+                }
+                stream.release();
+            }
+            if constexpr (Runs)
+                if (done > 0) take_back();
+#pragma unroll
+            for (int r = 0; r < S::kHalves; ++r) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                const int h = top_head + 8 * r;
+                const bool any = h < a.group && (!kQuarters || leads);
+                if (any && (lane & 3) == 0) {
+                    mine[h * width] = m[r];
+                    mine[h * width + 1] = l[r];
+                }
+#pragma unroll
+                for (int j = 0; j < DP / 8; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = o[j][2 * r + e];
+                        if constexpr (S::kPacked) x += o[j][2 + e];
+                        if constexpr (kQuarters) x += __shfl_xor_sync(0xffffffffu, x, 16);
+                        if (any && 8 * j < a.dim) mine[h * width + 2 + 8 * j + pair + e] = x;
+                    }
+            }
+            if constexpr (Runs) __syncwarp();
+            done += until;
+        } while (Runs && done < count);
         paged_join<Q, S::kTile, S::kWarps>(a, start, states, b, head, first, count, tiles, stream.now.left == 0);
     }
 }
 
-template <typename T, typename Q, int DP, int Heads>
+template <typename T, typename Q, int DP, int Heads, bool Runs>
 fx_status launch_mma(const PagedAttend& a, int sms, cudaStream_t stream) {
     using S = MmaShape<T, Q, DP, Heads>;
-    const fx_status st = raise_smem_limit(reinterpret_cast<const void*>(paged_mma_kernel<T, Q, DP, Heads>), S::kShared,
+    const auto kernel = paged_mma_kernel<T, Q, DP, Heads, Runs>;
+    const fx_status st = raise_smem_limit(reinterpret_cast<const void*>(kernel), S::kShared,
                                           "raising paged attention shared memory");
     if (st != FX_OK) return st;
     const int grid = paged_grid<S::kTile>(a, sms, S::kPerSm);
-    const fx_status launched = launch_dependent(paged_mma_kernel<T, Q, DP, Heads>, dim3(grid), dim3(S::kThreads),
-                                                S::kShared, stream, "launching paged attention", a);
+    const fx_status launched =
+        launch_dependent(kernel, dim3(grid), dim3(S::kThreads), S::kShared, stream, "launching paged attention", a);
     if (launched != FX_OK) return launched;
     return a.whole ? FX_OK : launch_paged_merge<Q>(a, grid, stream);
 }
 
-template <typename T, typename Q, int DP>
+template <typename T, typename Q, int DP, bool Runs>
 fx_status launch_mma_heads(const PagedAttend& a, int sms, cudaStream_t stream) {
     if constexpr (!std::is_same<T, Q>::value)
-        if (a.group <= 4) return launch_mma<T, Q, DP, 4>(a, sms, stream);
-    return a.group <= 8 ? launch_mma<T, Q, DP, 8>(a, sms, stream) : launch_mma<T, Q, DP, 16>(a, sms, stream);
+        if (a.group <= 4) return launch_mma<T, Q, DP, 4, false>(a, sms, stream);
+    return a.group <= 8 ? launch_mma<T, Q, DP, 8, Runs>(a, sms, stream)
+                        : launch_mma<T, Q, DP, 16, Runs>(a, sms, stream);
 }
+
+template <typename T, typename Q, bool Runs>
+fx_status launch_mma_dims(const PagedAttend& a, int sms, cudaStream_t stream) {
+    if (a.dim <= 64) return launch_mma_heads<T, Q, 64, Runs>(a, sms, stream);
+    if (a.dim <= 128) return launch_mma_heads<T, Q, 128, Runs>(a, sms, stream);
+    return launch_mma_heads<T, Q, 256, Runs>(a, sms, stream);
+}
+
+// A CTA may get all rows of a sequence.  1024 tiles in one sum lose 2^-14 on
+// average and 2^-12 at most, less than half a step of float16.  Kernels with runs
+// are larger, which short calls pay for (16 sequences of 200 rows: 10.3 us, 9.7
+// without), and otherwise 0-1 % slower.
+constexpr int kSumRows = 65536;
 
 template <typename T, typename Q>
 fx_status launch_mma_pages(const PagedAttend& a, int sms, cudaStream_t stream) {
-    if (a.dim <= 64) return launch_mma_heads<T, Q, 64>(a, sms, stream);
-    if (a.dim <= 128) return launch_mma_heads<T, Q, 128>(a, sms, stream);
-    return launch_mma_heads<T, Q, 256>(a, sms, stream);
+    if constexpr (std::is_same<T, Q>::value)
+        if (a.capacity > kSumRows) return launch_mma_dims<T, Q, true>(a, sms, stream);
+    return launch_mma_dims<T, Q, false>(a, sms, stream);
 }
 
 }  // namespace fx

@@ -85,3 +85,42 @@ def test_attention_with_the_largest_queries_on_16_bit_pages(group):
     k[..., :4] = k[..., :4].sign() * 2.0 ** -126
     out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lengths.cuda(), 0.25)
     _assert_attention(out, q, k, v, table, lengths, 0.25)
+
+
+@pytest.mark.parametrize("dim,group", [(64, 4), (128, 8), (256, 3), (64, 16), (128, 9)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", [(1 << 21) + 64 * 255, (1 << 16) + 64, 1 << 16, 1 << 14])
+def test_attention_sums_over_millions_of_rows(dtype, dim, group, rows):
+    """Values of one sign, equal weights, whole units in one CTA each: what is lost at every step would add up."""
+    page, batch = 64, 112  # 448 units
+    v = (_randn((1, 4, page, dim), torch.float32, 2).abs() + 0.5).to(dtype)
+    k = torch.zeros_like(v)
+    q = _randn((batch, 4 * group, 1, dim), dtype, 3)
+    table = torch.zeros((1, rows // page), dtype=torch.int32, device="cuda").expand(batch, -1).contiguous()
+    lengths = torch.full((batch,), rows, device="cuda")
+    out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table, lengths, 0.1).cpu().double()
+    expected = v[0].double().mean(1).repeat_interleave(group, 0).view(1, 4 * group, 1, dim)
+    # 2 terms of a run's tiles truncated by less than 2^-23 each, then float32 sums of the runs (of 256 tiles beyond
+    # 65536 rows), and the weights' terms; one rounding to 16 bits
+    run = 256 if rows > 1 << 16 else rows // page
+    tolerance = 2 * run * 2.0 ** -23 + rows // page / run * ref.U32 + 2.0 ** -16 + 1.01 * ref.half_step(dtype)
+    error = ((out - expected).abs() / expected).max().item()
+    assert error <= tolerance, (error, tolerance)
+
+
+@pytest.mark.parametrize("query", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("group", [3, 8, 12])
+@pytest.mark.parametrize("columns", [600, 1100])
+def test_attention_joins_runs_of_any_maximum(query, group, columns):
+    """More tiles in one CTA than are summed in one go, whose scores rise, fall, or are hidden for long."""
+    page, pages, batch, rows = 64, 40, 160, 600 * 64
+    k, v = (_randn((pages, 3, page, 64), TYPES[query], seed) for seed in (1, 2))
+    k *= torch.linspace(0.1, 3, pages).view(-1, 1, 1, 1).to(k.dtype)
+    q = _randn((batch, 3 * group, 1, 64), TYPES[query], 3)
+    order = torch.arange(600) * pages // 600
+    table = torch.stack([order, order.flip(0), torch.where(order < 20, -1, order), torch.where(order < 35, order, -1)])
+    table = torch.nn.functional.pad(table, (0, columns - 600), value=-1).int().repeat(batch // 4, 1)
+    lengths = torch.full((batch,), rows - 17)
+    out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lengths.cuda(), 0.125)
+    pick = [0, 1, 2, 3, 156, 157, 158, 159]
+    _assert_attention(out[pick], q[pick], k, v, table[pick], lengths[pick], 0.125)
