@@ -69,7 +69,9 @@ int* decode_error_word(fx_decode* runtime);
 // is scheduled as the previous kernel in the stream retires its CTAs; it
 // calls grid_dependency_wait() before touching anything that kernel produced
 // (a no-op for an ordinary launch).  Kernels do not trigger their successors
-// early: measured, an early trigger slowed the batched step.
+// early: measured, an early trigger slowed the batched step.  The one exception
+// is paged attention before its merge, whose every thread waits first, so that
+// whatever is launched behind the merge finds both complete.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Scheduling priority given to this thread's launch_dependent() launches

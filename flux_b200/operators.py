@@ -936,7 +936,7 @@ def paged_qkv_rope_cache_native(packed_qkv, cos, sin, key_pages, value_pages, pa
 
 def paged_gqa_decode_attention_native(query, key_pages, value_pages, page_table, lengths, scale):
     """One-token attention ``[B, Hq, 1, D]`` of every sequence over its first ``lengths[b]`` rows in the pages; rows of
-    holes are hidden, and a sequence without a visible row gives zeros."""
+    holes are hidden, and a sequence without a visible row (or whose scores are all -inf) gives zeros."""
     _require_serving("paged GQA decode attention")
     return torch.ops.flux.paged_gqa_decode_attention(query, key_pages, value_pages, page_table, lengths, scale)
 

@@ -255,8 +255,13 @@ FX_API fx_status fx_paged_qkv_rope_cache(const void* packed_qkv, int32_t dtype, 
  * out[b, h] = sum_r softmax_r(scale * query[b, h] . K[r]) V[r] over the rows
  * r < lengths[b] (clamped to [0, table_columns * page_size]) outside holes, of
  * KV head h / (query_heads / kv_heads).  A sequence with no visible row gives
- * zeros.  A NaN in a visible row is passed on, and an infinity there gives a
- * result that is not finite.  query [batch, query_heads, head_dim] (strides of
+ * zeros.  A NaN in a visible row is passed on.  An infinity in a visible value
+ * row gives a result that is not finite.  One in a key row gives a score of +inf,
+ * hence NaN, or of -inf, hence weight 0 (zeros where all scores are -inf, as they
+ * also are when finite products leave FP32's range that way); FP32 queries on
+ * 16-bit pages may give NaN instead.  Scores and sums are FP32: values whose sum
+ * over the rows, before it is divided, leaves its range give infinities.
+ * query [batch, query_heads, head_dim] (strides of
  * batch and head in elements, rows contiguous) and the contiguous output have
  * type dtype: FX_F32 with pages of any type, or the pages' own type.  Up to 16
  * query heads per KV head are read for at once; of more, the largest part that

@@ -124,3 +124,45 @@ def test_attention_joins_runs_of_any_maximum(query, group, columns):
     out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lengths.cuda(), 0.125)
     pick = [0, 1, 2, 3, 156, 157, 158, 159]
     _assert_attention(out[pick], q[pick], k, v, table[pick], lengths[pick], 0.125)
+
+
+INF = float("inf")
+
+
+@pytest.mark.parametrize("query,pages,group", [("f32", "f32", 1), ("f32", "f32", 4), ("f32", "f32", 5), ("f32", "f32", 16),
+                                               ("f32", "bf16", 3), ("f32", "f16", 9), ("bf16", "bf16", 2), ("f16", "f16", 16)])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("length", [1, 100])
+def test_attention_with_an_infinity_in_a_key_row(query, pages, group, sign, length):
+    """A score of -inf has weight 0 (zeros where all scores are); one of +inf gives NaN.  Float32 queries meet 16-bit
+    keys as terms, one of which may be 0: NaN either way."""
+    k, v = (_randn((8, 1, 16, 64), TYPES[pages], seed) for seed in (1, 2))
+    q = _randn((1, group, 1, 64), TYPES[query], 3).abs() + 0.5
+    q = q.to(TYPES[query])
+    table = torch.arange(7, dtype=torch.int32).view(1, -1)
+    k[0, 0, 0, 5] = sign * INF
+    out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(),
+                                                   torch.tensor([length], device="cuda"), 0.125).cpu()
+    if sign > 0:
+        assert out.isnan().all()
+    elif query == pages and length == 1:
+        assert not out.any()
+    elif query == pages:
+        k[0, 0, 0] = -(q[0, 0, 0].float() * 1e4).to(k.dtype)  # as far below the others as to have no weight
+        _assert_attention(out, q, k, v, table, torch.tensor([length]), 0.125)
+    else:
+        assert out.isnan().all() or out.isfinite().all()
+
+
+@pytest.mark.parametrize("query,pages,group", [("f32", "f32", 4), ("f32", "f32", 5), ("f32", "f32", 16), ("f32", "f16", 9),
+                                               ("bf16", "bf16", 2)])
+@pytest.mark.parametrize("size", [INF, -INF, float("nan")])
+def test_attention_with_an_infinity_in_a_value_row(query, pages, group, size):
+    """Not finite where the row counts, in its own dim only."""
+    k, v = (_randn((8, 1, 16, 64), TYPES[pages], seed) for seed in (1, 2))
+    q = _randn((1, group, 1, 64), TYPES[query], 3)
+    v[3, 0, 7, 9] = size
+    table = torch.arange(7, dtype=torch.int32).view(1, -1)
+    out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(),
+                                                   torch.tensor([100], device="cuda"), 0.125).cpu()
+    assert not out[..., 9].isfinite().any() and out[..., :9].isfinite().all() and out[..., 10:].isfinite().all()
