@@ -7,6 +7,8 @@
 // One function serves the CUDA, CPU and Meta keys.  It checks its arguments
 // first, on any device; then a CUDA call launches, a Meta call (FakeTensor)
 // returns the shapes, and a CPU call is refused: there is no CPU compute path.
+// A Meta call whose sizes are symbols goes to a function of its own, which checks
+// ranks, types and sizes and keeps the symbols.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDACachingAllocator.h>
@@ -460,6 +462,253 @@ Tensor logits_process_out(const Tensor& logits, const Optional& tokens, const Op
     return out;
 }
 
+// --------------------------------------------------- sizes that are symbols
+
+bool symbolic(std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors)
+        if (t->unsafeGetTensorImpl()->has_symbolic_sizes_strides()) return true;
+    return false;
+}
+
+const Tensor* given(const Optional& t, const Tensor& otherwise) { return t.has_value() ? &*t : &otherwise; }
+
+void symbolic_pages(const char* op, const Tensor& keys, const Tensor& values, int64_t rank) {
+    TORCH_CHECK(keys.dim() == rank && values.dim() == rank, op, ": key_pages and value_pages must be ",
+                rank == 5 ? "[layers, pages, kv_heads, page_size, head_dim]" : "[pages, kv_heads, page_size, head_dim]");
+    for (int64_t d = 0; d < rank; ++d)
+        TORCH_SYM_CHECK(keys.sym_size(d).sym_eq(values.sym_size(d)), op,
+                        ": key_pages and value_pages must have the same shape");
+    TORCH_CHECK(keys.scalar_type() == values.scalar_type(), op, ": key_pages and value_pages must have the same type");
+    dtype_of(op, keys, "key_pages");
+    const c10::SymInt dim = keys.sym_size(rank - 1);
+    TORCH_SYM_CHECK((dim % 8).sym_eq(0).sym_and(dim.sym_le(256)), op, ": head_dim must be a multiple of 8 up to 256");
+    no_grad(op, {&keys, &values});
+}
+
+void symbolic_table(const char* op, const Tensor& t) {
+    TORCH_CHECK(t.dim() == 2 && t.scalar_type() == at::kInt, op, ": page_table must be a two-dimensional int32 tensor");
+}
+
+void symbolic_vector(const char* op, const Tensor& t, const char* name, const c10::SymInt& size) {
+    TORCH_CHECK(t.dim() == 1 && t.scalar_type() == at::kLong, op, ": ", name,
+                " must be a contiguous one-dimensional int64 tensor");
+    TORCH_SYM_CHECK(t.sym_size(0).sym_eq(size), op, ": ", name, " has another number of entries than expected");
+}
+
+void symbolic_state(const char* op, const Tensor& table, const Tensor& counts) {
+    symbolic_table(op, table);
+    TORCH_CHECK(counts.dim() == 1 && counts.scalar_type() == at::kInt, op,
+                ": page_counts must be a contiguous one-dimensional int32 tensor");
+}
+
+Tensor paged_qkv_rope_cache_meta(const Tensor& packed, const Tensor& cos, const Tensor& sin, const Tensor& keys,
+                                 const Tensor& values, const Tensor& table, const Tensor& positions,
+                                 const Optional& sequences) {
+    const char* op = "flux::paged_qkv_rope_cache";
+    if (!symbolic({&packed, &cos, &sin, &keys, &values, &table, &positions, given(sequences, positions)}))
+        return paged_qkv_rope_cache(packed, cos, sin, keys, values, table, positions, sequences);
+    symbolic_pages(op, keys, values, 4);
+    symbolic_table(op, table);
+    const char* shape = ": packed_qkv must be [tokens, (query_heads + 2 kv_heads) * head_dim]";
+    TORCH_CHECK(packed.dim() == 2, op, shape);
+    const c10::SymInt tokens = packed.sym_size(0), width = packed.sym_size(1), dim = keys.sym_size(3);
+    TORCH_SYM_CHECK((width % dim).sym_eq(0), op, shape);
+    const c10::SymInt heads = width / dim - keys.sym_size(1) * 2;
+    TORCH_SYM_CHECK(heads.sym_gt(0), op, shape);
+    TORCH_CHECK(packed.scalar_type() == at::kFloat || packed.scalar_type() == keys.scalar_type(), op,
+                ": packed_qkv must be float32 or have the pages' type");
+    TORCH_CHECK(cos.dim() == 2 && sin.dim() == 2, op, ": cos and sin must be tables [positions, head_dim]");
+    TORCH_SYM_CHECK(cos.sym_size(0).sym_eq(sin.sym_size(0)).sym_and(cos.sym_size(1).sym_eq(dim))
+                        .sym_and(sin.sym_size(1).sym_eq(dim)),
+                    op, ": cos and sin must be tables [positions, head_dim]");
+    TORCH_CHECK(cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat, op,
+                ": cos and sin must be float32 with contiguous rows");
+    symbolic_vector(op, positions, "positions", tokens);
+    if (sequences.has_value())
+        symbolic_vector(op, *sequences, "sequences", tokens);
+    else
+        TORCH_SYM_CHECK(tokens.sym_eq(table.sym_size(0)), op, ": without sequences there is one token per page_table row");
+    same_device(op, keys, {&values, &packed, &cos, &sin, &table, &positions, given(sequences, positions)});
+    no_grad(op, {&packed, &cos, &sin});
+    return at::empty_symint({tokens, heads, 1, dim}, packed.options());
+}
+
+void symbolic_attend(const char* op, const Tensor& query, const Tensor& keys, const Tensor& values, const Tensor& table,
+                     const Tensor& lengths, double scale) {
+    symbolic_pages(op, keys, values, 4);
+    TORCH_CHECK(query.dim() == 4, op, ": query must be [batch, query_heads, 1, head_dim]");
+    TORCH_SYM_CHECK(query.sym_size(2).sym_eq(1), op, ": query must be [batch, query_heads, 1, head_dim]");
+    symbolic_table(op, table);
+    TORCH_SYM_CHECK(query.sym_size(3).sym_eq(keys.sym_size(3)), op, ": cache head dimension must match query");
+    TORCH_SYM_CHECK((query.sym_size(1) % keys.sym_size(1)).sym_eq(0), op, ": query heads must be divisible by KV heads");
+    TORCH_CHECK(query.scalar_type() == at::kFloat || query.scalar_type() == keys.scalar_type(), op,
+                ": query must be float32 or have the pages' type");
+    TORCH_SYM_CHECK(query.sym_size(0).sym_eq(table.sym_size(0)), op,
+                    ": page_table must have one row per sequence of the query");
+    symbolic_vector(op, lengths, "lengths", query.sym_size(0));
+    TORCH_CHECK(std::isfinite(scale) && std::isfinite(static_cast<float>(scale)), op,
+                ": scale must be a finite FP32 value");
+    same_device(op, query, {&keys, &values, &table, &lengths});
+    no_grad(op, {&query});
+}
+
+Tensor paged_gqa_decode_attention_meta(const Tensor& query, const Tensor& keys, const Tensor& values,
+                                       const Tensor& table, const Tensor& lengths, double scale) {
+    if (!symbolic({&query, &keys, &values, &table, &lengths}))
+        return paged_gqa_decode_attention(query, keys, values, table, lengths, scale);
+    symbolic_attend("flux::paged_gqa_decode_attention", query, keys, values, table, lengths, scale);
+    return at::empty_symint(query.sym_sizes(), query.options());
+}
+
+void symbolic_output(const char* op, const Tensor& output, const Tensor& like, const char* message) {
+    TORCH_CHECK(output.dim() == like.dim() && output.scalar_type() == like.scalar_type(), op, message);
+    for (int64_t d = 0; d < like.dim(); ++d)
+        TORCH_SYM_CHECK(output.sym_size(d).sym_eq(like.sym_size(d)), op, message);
+    same_device(op, like, {&output});
+    no_grad(op, {&output});
+}
+
+Tensor paged_gqa_decode_attention_out_meta(const Tensor& query, const Tensor& keys, const Tensor& values,
+                                           const Tensor& table, const Tensor& lengths, double scale,
+                                           const Tensor& output, const Tensor& workspace) {
+    const char* op = "flux::paged_gqa_decode_attention_out";
+    if (!symbolic({&query, &keys, &values, &table, &lengths, &output, &workspace}))
+        return paged_gqa_decode_attention_out(query, keys, values, table, lengths, scale, output, workspace);
+    symbolic_attend(op, query, keys, values, table, lengths, scale);
+    symbolic_output(op, output, query, ": output must have the shape and type of query");
+    TORCH_CHECK(workspace.scalar_type() == at::kFloat, op, ": workspace must be contiguous float32");
+    return output;
+}
+
+void cache_pages_copy_meta(const Tensor& keys, const Tensor& values, const Tensor& source, const Tensor& destination) {
+    const char* op = "flux::cache_pages_copy";
+    if (!symbolic({&keys, &values, &source, &destination})) return cache_pages_copy(keys, values, source, destination);
+    symbolic_pages(op, keys, values, 5);
+    TORCH_CHECK(source.dim() == 1, op, ": source must be a contiguous one-dimensional int64 tensor");
+    symbolic_vector(op, source, "source", source.sym_size(0));
+    symbolic_vector(op, destination, "destination", source.sym_size(0));
+    same_device(op, keys, {&values, &source, &destination});
+}
+
+Tensor cache_sequences_reserve_meta(const Tensor& table, const Tensor& lengths, const Tensor& counts,
+                                    const Tensor& sequences, const Tensor& rows, int64_t page_size) {
+    const char* op = "flux::cache_sequences_reserve";
+    if (!symbolic({&table, &lengths, &counts, &sequences, &rows}))
+        return cache_sequences_reserve(table, lengths, counts, sequences, rows, page_size);
+    symbolic_state(op, table, counts);
+    symbolic_vector(op, lengths, "lengths", table.sym_size(0));
+    TORCH_CHECK(sequences.dim() == 1, op, ": sequences must be a contiguous one-dimensional int64 tensor");
+    symbolic_vector(op, sequences, "sequences", sequences.sym_size(0));
+    symbolic_vector(op, rows, "rows", sequences.sym_size(0));
+    TORCH_CHECK(page_size > 0, op, ": page_size must be positive");
+    same_device(op, table, {&lengths, &counts, &sequences, &rows});
+    return at::empty_symint({sequences.sym_size(0)}, counts.options());
+}
+
+Tensor cache_sequences_fork_meta(const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths,
+                                 const Tensor& counts, const Tensor& parents, const Tensor& children) {
+    const char* op = "flux::cache_sequences_fork";
+    if (!symbolic({&keys, &values, &table, &lengths, &counts, &parents, &children}))
+        return cache_sequences_fork(keys, values, table, lengths, counts, parents, children);
+    symbolic_pages(op, keys, values, 5);
+    symbolic_state(op, table, counts);
+    TORCH_SYM_CHECK(counts.sym_size(0).sym_eq(keys.sym_size(1)), op, ": page_counts must have one entry per page");
+    symbolic_vector(op, lengths, "lengths", table.sym_size(0));
+    TORCH_CHECK(parents.dim() == 1, op, ": parents must be a contiguous one-dimensional int64 tensor");
+    symbolic_vector(op, parents, "parents", parents.sym_size(0));
+    symbolic_vector(op, children, "children", parents.sym_size(0));
+    same_device(op, keys, {&values, &table, &lengths, &counts, &parents, &children});
+    return at::empty_symint({parents.sym_size(0)}, counts.options());
+}
+
+void cache_sequences_free_meta(const Tensor& table, const Tensor& lengths, const Tensor& counts,
+                               const Tensor& sequences) {
+    const char* op = "flux::cache_sequences_free";
+    if (!symbolic({&table, &lengths, &counts, &sequences}))
+        return cache_sequences_free(table, lengths, counts, sequences);
+    symbolic_state(op, table, counts);
+    symbolic_vector(op, lengths, "lengths", table.sym_size(0));
+    TORCH_CHECK(sequences.dim() == 1, op, ": sequences must be a contiguous one-dimensional int64 tensor");
+    symbolic_vector(op, sequences, "sequences", sequences.sym_size(0));
+    same_device(op, table, {&lengths, &counts, &sequences});
+}
+
+Tensor cache_pages_compact_meta(const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& counts) {
+    const char* op = "flux::cache_pages_compact";
+    if (!symbolic({&keys, &values, &table, &counts})) return cache_pages_compact(keys, values, table, counts);
+    symbolic_pages(op, keys, values, 5);
+    symbolic_state(op, table, counts);
+    TORCH_SYM_CHECK(counts.sym_size(0).sym_eq(keys.sym_size(1)), op, ": page_counts must have one entry per page");
+    same_device(op, keys, {&values, &table, &counts});
+    return at::empty({}, counts.options());
+}
+
+// [width], [1, width] or [rows, width]
+void symbolic_row(const char* op, const Tensor& t, const char* name, const c10::SymInt& rows, const c10::SymInt& width) {
+    TORCH_CHECK(t.dim() == 1 || t.dim() == 2, op, ": ", name, " must be one row or one row per row of logits");
+    c10::SymBool fits = t.sym_size(t.dim() - 1).sym_eq(width);
+    if (t.dim() == 2) fits = fits.sym_and(t.sym_size(0).sym_eq(1).sym_or(t.sym_size(0).sym_eq(rows)));
+    TORCH_SYM_CHECK(fits, op, ": ", name, " must be one row or one row per row of logits, as wide as they are");
+}
+
+bool symbolic_logits(const char* op, const Tensor& logits, const Optional& tokens, const Optional& prompt_lengths,
+                     const Optional& lengths, const Optional& penalties, const Optional& bias, const Optional& allowed,
+                     const Tensor& output) {
+    if (!symbolic({&logits, &output, given(tokens, logits), given(prompt_lengths, logits), given(lengths, logits),
+                   given(penalties, logits), given(bias, logits), given(allowed, logits)}))
+        return false;
+    TORCH_CHECK(logits.dim() == 2, op, ": logits must be [rows, vocabulary]");
+    dtype_of(op, logits, "logits");
+    const c10::SymInt rows = logits.sym_size(0), vocab = logits.sym_size(1);
+    const bool history = tokens.has_value();
+    TORCH_CHECK(history == prompt_lengths.has_value() && history == lengths.has_value() &&
+                    history == penalties.has_value(),
+                op, ": tokens, prompt_lengths, lengths and penalties go together");
+    if (history) {
+        TORCH_CHECK(tokens->dim() == 2 && tokens->scalar_type() == at::kLong, op, ": tokens must be int64 [rows, history]");
+        TORCH_SYM_CHECK(tokens->sym_size(0).sym_eq(rows), op, ": tokens must be int64 [rows, history]");
+        symbolic_vector(op, *prompt_lengths, "prompt_lengths", rows);
+        symbolic_vector(op, *lengths, "lengths", rows);
+        TORCH_CHECK(penalties->dim() == 2 && penalties->scalar_type() == at::kFloat, op,
+                    ": penalties must be contiguous float32 [rows, 3]");
+        TORCH_SYM_CHECK(penalties->sym_size(0).sym_eq(rows).sym_and(penalties->sym_size(1).sym_eq(3)), op,
+                        ": penalties must be contiguous float32 [rows, 3]");
+        no_grad(op, {&*penalties});
+    }
+    if (bias.has_value()) {
+        TORCH_CHECK(bias->scalar_type() == at::kFloat, op, ": bias must be float32");
+        symbolic_row(op, *bias, "bias", rows, vocab);
+        no_grad(op, {&*bias});
+    }
+    if (allowed.has_value()) {
+        TORCH_CHECK(allowed->scalar_type() == at::kInt, op, ": allowed must be int32 words of 32 token bits");
+        symbolic_row(op, *allowed, "allowed", rows, (vocab + 31) / 32);
+    }
+    same_device(op, logits, {given(tokens, logits), given(prompt_lengths, logits), given(lengths, logits),
+                             given(penalties, logits), given(bias, logits), given(allowed, logits)});
+    no_grad(op, {&logits});
+    return true;
+}
+
+Tensor logits_process_meta(const Tensor& logits, const Optional& tokens, const Optional& prompt_lengths,
+                           const Optional& lengths, const Optional& penalties, const Optional& bias,
+                           const Optional& allowed) {
+    if (!symbolic_logits("flux::logits_process", logits, tokens, prompt_lengths, lengths, penalties, bias, allowed,
+                         logits))
+        return logits_process(logits, tokens, prompt_lengths, lengths, penalties, bias, allowed);
+    return at::empty_symint(logits.sym_sizes(), logits.options());
+}
+
+Tensor logits_process_out_meta(const Tensor& logits, const Optional& tokens, const Optional& prompt_lengths,
+                               const Optional& lengths, const Optional& penalties, const Optional& bias,
+                               const Optional& allowed, const Tensor& output) {
+    const char* op = "flux::logits_process_out";
+    if (!symbolic_logits(op, logits, tokens, prompt_lengths, lengths, penalties, bias, allowed, output))
+        return logits_process_out(logits, tokens, prompt_lengths, lengths, penalties, bias, allowed, output);
+    symbolic_output(op, output, logits, ": output must have the shape and type of logits");
+    return output;
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(flux, m) {
@@ -484,18 +733,18 @@ TORCH_LIBRARY_FRAGMENT(flux, m) {
           "Tensor? penalties, Tensor? bias, Tensor? allowed, Tensor(a!) output) -> Tensor(a!)");
 }
 
-#define FLUX_SERVING_OPERATORS(m)                                                  \
-    m.impl("paged_qkv_rope_cache", TORCH_FN(paged_qkv_rope_cache));                \
-    m.impl("paged_gqa_decode_attention", TORCH_FN(paged_gqa_decode_attention));    \
-    m.impl("paged_gqa_decode_attention_out", TORCH_FN(paged_gqa_decode_attention_out)); \
-    m.impl("cache_pages_copy", TORCH_FN(cache_pages_copy));                        \
-    m.impl("cache_sequences_reserve", TORCH_FN(cache_sequences_reserve));          \
-    m.impl("cache_sequences_fork", TORCH_FN(cache_sequences_fork));                \
-    m.impl("cache_sequences_free", TORCH_FN(cache_sequences_free));                \
-    m.impl("cache_pages_compact", TORCH_FN(cache_pages_compact));                  \
-    m.impl("logits_process", TORCH_FN(logits_process));                            \
-    m.impl("logits_process_out", TORCH_FN(logits_process_out))
+#define FLUX_SERVING_OPERATORS(m, form) \
+    m.impl("paged_qkv_rope_cache", TORCH_FN(paged_qkv_rope_cache##form)); \
+    m.impl("paged_gqa_decode_attention", TORCH_FN(paged_gqa_decode_attention##form)); \
+    m.impl("paged_gqa_decode_attention_out", TORCH_FN(paged_gqa_decode_attention_out##form)); \
+    m.impl("cache_pages_copy", TORCH_FN(cache_pages_copy##form)); \
+    m.impl("cache_sequences_reserve", TORCH_FN(cache_sequences_reserve##form)); \
+    m.impl("cache_sequences_fork", TORCH_FN(cache_sequences_fork##form)); \
+    m.impl("cache_sequences_free", TORCH_FN(cache_sequences_free##form)); \
+    m.impl("cache_pages_compact", TORCH_FN(cache_pages_compact##form)); \
+    m.impl("logits_process", TORCH_FN(logits_process##form)); \
+    m.impl("logits_process_out", TORCH_FN(logits_process_out##form))
 
-TORCH_LIBRARY_IMPL(flux, CUDA, m) { FLUX_SERVING_OPERATORS(m); }
-TORCH_LIBRARY_IMPL(flux, CPU, m) { FLUX_SERVING_OPERATORS(m); }
-TORCH_LIBRARY_IMPL(flux, Meta, m) { FLUX_SERVING_OPERATORS(m); }
+TORCH_LIBRARY_IMPL(flux, CUDA, m) { FLUX_SERVING_OPERATORS(m, ); }
+TORCH_LIBRARY_IMPL(flux, CPU, m) { FLUX_SERVING_OPERATORS(m, ); }
+TORCH_LIBRARY_IMPL(flux, Meta, m) { FLUX_SERVING_OPERATORS(m, _meta); }
