@@ -57,11 +57,16 @@ void same_device(const char* op, const Tensor& first, std::initializer_list<cons
 }
 
 void no_grad(const char* op, std::initializer_list<const Tensor*> tensors) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor* t : tensors)
-        TORCH_CHECK(!t->requires_grad(), op,
+    const bool backward = at::GradMode::is_enabled();
+    const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    if (!backward && !forward) return;
+    for (const Tensor* t : tensors) {
+        TORCH_CHECK(!backward || !t->requires_grad(), op,
                     " is inference-only; use torch.no_grad() or torch.inference_mode() for tensors that require "
                     "gradients");
+        TORCH_CHECK(!forward || !t->_fw_grad(0).defined(), op,
+                    " is inference-only; it has no forward-mode derivative");
+    }
 }
 
 int32_t dtype_of(const char* op, const Tensor& t, const char* name) {

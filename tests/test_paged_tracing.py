@@ -1,10 +1,11 @@
 """The paged-cache and logits operators under tracing with sizes that may
-change.  No call here reaches CUDA."""
+change, and under forward-mode differentiation.  No call here reaches CUDA."""
 
 from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 from torch._subclasses.fake_tensor import FakeTensorMode
 from torch.fx.experimental.symbolic_shapes import DimDynamic, ShapeEnv, StatelessSymbolicContext
 
@@ -114,3 +115,21 @@ def test_a_traced_step_serves_other_batches():
     graph = make_fx(step, tracing_mode="symbolic")(*args)
     values = [n.meta["val"] for n in graph.graph.nodes if n.op == "call_function" and "val" in n.meta]
     assert values and all(is_symbol(v.shape[0]) for v in values if isinstance(v, torch.Tensor))
+
+
+def test_forward_mode_derivatives_are_refused():
+    x, t = torch.zeros(2, 100), torch.ones(2, 100)
+    k, v = torch.zeros(5, 2, 16, 64), torch.zeros(5, 2, 16, 64)
+    table, lengths = torch.zeros((2, 3), dtype=torch.int32), torch.zeros(2, dtype=torch.int64)
+    with forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="inference-only"):
+            ops.logits_process_native(forward_ad.make_dual(x, t))
+        q = torch.zeros(2, 6, 1, 64)
+        with pytest.raises(RuntimeError, match="inference-only"):
+            ops.paged_gqa_decode_attention_native(forward_ad.make_dual(q, q + 1), k, v, table, lengths, 0.125)
+        with pytest.raises(RuntimeError, match="inference-only"):
+            ops.paged_gqa_decode_attention_native(q, k, forward_ad.make_dual(v, v + 1), table, lengths, 0.125)
+        with pytest.raises(RuntimeError, match="CUDA tensors are required"):
+            ops.logits_process_native(x)
+    with pytest.raises(RuntimeError, match="CUDA tensors are required"):
+        ops.logits_process_native(x)
