@@ -53,16 +53,30 @@ struct Penalties { float repetition, inverse, presence, frequency; };
 
 __device__ __forceinline__ Penalties penalties_of(const LogitsArgs& a, int row) {
     const float* p = a.penalties + 3 * static_cast<int64_t>(row);
-    return {p[0], 1.0f / p[0], p[1], p[2]};
+    return {p[0], __frcp_rn(p[0]), p[1], p[2]};
 }
 
-// FP32 in the order of the definition.  x / repetition is taken as the product
-// with the row's reciprocal, which is off by at most one step of FP32 more (and
-// exact for repetition 1); the product that the frequency adds is rounded on
-// its own, as are the differences.
-template <typename C>
+// FP32 in the order of the definition: a division or a product, then the product
+// that the frequency adds and two differences, each rounded on its own.
+//
+// The quotient: with the divisor's reciprocal y rounded to nearest, q = x y and
+// its remainder r = x - q d, which a fused product gives exactly, q + r y is the
+// quotient rounded to nearest (Markstein, 1990), except for divisors whose
+// mantissa is all ones or whose reciprocal is no normal number: off by one step of
+// FP32 at most there.  A division per seen logit would be slower (1 x 49152 FP32
+// logits 5.5 us, 4.8 in this way).  16-bit logits take q as it is: one step of FP32
+// is far below their own rounding (256 x 100277 BF16 logits 55.5 us, 57.2 with the
+// remainder).
+template <typename T>
+__device__ __forceinline__ float divided(float x, const Penalties& p) {
+    const float q = x * p.inverse;
+    if constexpr (sizeof(T) == 2) return q;
+    const float near = fmaf(fmaf(-q, p.repetition, x), p.inverse, q);
+    return q < INFINITY ? near : q;  // an infinite q has no remainder
+}
+template <typename T, typename C>
 __device__ __forceinline__ float penalised(float x, uint32_t count, const Penalties& p) {
-    x *= x > 0.0f ? p.inverse : p.repetition;
+    x = x > 0.0f ? divided<T>(x, p) : x * p.repetition;
     const uint32_t n = count & (kPrompt<C> - 1u);
     if (n != 0u) x = __fsub_rn(__fsub_rn(x, __fmul_rn(p.frequency, static_cast<float>(n))), p.presence);
     return x;
@@ -136,7 +150,7 @@ __device__ __forceinline__ void replace(const Part<T>& part, const uint4& raw, u
         const uint16_t bits = static_cast<uint16_t>(half);
         x = to_float(*reinterpret_cast<const T*>(&bits));
     }
-    x = penalised<C>(x, count, p);
+    x = penalised<T, C>(x, count, p);
     if (part.bias != nullptr) x += part.bias[at + e];
     part.out[at + e] = from_float<T>((mask >> e) & 1u ? x : -INFINITY);
 }
@@ -205,7 +219,7 @@ __device__ __forceinline__ void process(const Part<T>& part, void* counters, con
         if constexpr (kHistory) {
             const uint32_t c = counts[at];
             if (c != 0u) {
-                v = penalised<C>(v, c, p);
+                v = penalised<T, C>(v, c, p);
                 counts[at] = 0;
             }
         }

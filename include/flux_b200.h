@@ -329,7 +329,7 @@ FX_API fx_status fx_cache_pages_compact(const fx_pages* pages, int32_t* page_tab
 /* Penalties, bias and token mask on logits [rows, vocab] of type dtype, in FP32
  * with one rounding at the end (output may be the input itself):
  *   x = logits[b, v]
- *   x = x > 0 ? x * (1 / repetition) : x * repetition  if v is in tokens[b, :lengths[b]]
+ *   x = x > 0 ? x / repetition : x * repetition  if v is in tokens[b, :lengths[b]]
  *   x = x - frequency * n - presence * (n > 0),  n = times v is in
  *                                  tokens[b, prompt_lengths[b]:lengths[b]]
  *   x = x + bias[b, v]
@@ -339,7 +339,8 @@ FX_API fx_status fx_cache_pages_compact(const fx_pages* pages, int32_t* page_tab
  * to [0, history], prompt lengths to [0, length]; tokens outside [0, vocab)
  * are ignored.  bias and allowed may be NULL; a row stride of 0 broadcasts
  * them.  Without an allowed token a row is all -inf.  fx_greedy_argmax_f32
- * takes the result. */
+ * takes the result.  With 16-bit logits the quotient may be off by one step of
+ * FP32. */
 FX_API fx_status fx_logits_process(const void* logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t logits_stride,
                             const int64_t* tokens, int64_t history, int64_t tokens_stride,
                             const int64_t* prompt_lengths, const int64_t* lengths, const float* penalties,

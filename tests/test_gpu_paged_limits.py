@@ -166,3 +166,40 @@ def test_attention_with_an_infinity_in_a_value_row(query, pages, group, size):
     out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(),
                                                    torch.tensor([100], device="cuda"), 0.125).cpu()
     assert not out[..., 9].isfinite().any() and out[..., :9].isfinite().all() and out[..., 10:].isfinite().all()
+
+
+@pytest.mark.parametrize("vocab,history", [(33, 40), (8193, 9000), (30001, 40000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_penalties_are_those_of_float32(dtype, vocab, history):
+    """Bit for bit: a division or a product, a product, two differences and a sum, each rounded once in float32.  16-bit
+    logits, whose quotient may be off by one step of float32, are rounded once more from there."""
+    g = torch.Generator().manual_seed(vocab)
+    repetition = torch.tensor([1.1, 1.3, 0.7, 3.0, 1e-20, 1e20, 1.0000001, 1.9999998])
+    rows = repetition.shape[0]
+    x = (torch.randn((rows, vocab), generator=g) * 3).to(dtype)
+    x[3, :9] = torch.tensor([float("inf"), -float("inf"), 3.3e38, -3.3e38, 0.0, -0.0, 1e-30, 1e30, 2.0 ** 120])
+    tokens_of_row_3 = torch.arange(9)
+    tokens = torch.randint(vocab, (rows, history), generator=g)
+    tokens[3, :9] = tokens_of_row_3
+    lengths = torch.full((rows,), history - 3)
+    prompts = torch.tensor([0, 5, history, 7, history, history, 11, 9])
+    bias = torch.randn(vocab, generator=g)
+    penalties = torch.stack((repetition, torch.rand(rows, generator=g), torch.rand(rows, generator=g)), 1)
+    out = _ops().logits_process_native(x.cuda(), tokens.cuda(), prompts.cuda(), lengths.cuda(), penalties.cuda(), bias.cuda())
+    column = torch.arange(history)
+    inside = (column < lengths.unsqueeze(1)).float()
+    emitted = inside * (column >= prompts.unsqueeze(1))
+    zero = torch.zeros((rows, vocab))
+    seen, count = zero.scatter_add(1, tokens, inside) > 0, zero.scatter_add(1, tokens, emitted)
+    r, presence, frequency = penalties.unsqueeze(2).unbind(1)
+    y = x.float()
+    y = torch.where(seen, torch.where(y > 0, y / r, y * r), y)
+    y = torch.where(count > 0, y - frequency * count - presence, y) + bias
+    if dtype == torch.float32:
+        assert torch.equal(out.cpu(), y)
+        return
+    got, size = out.cpu().double(), torch.maximum(x.double().abs() / r.double(), y.double().abs())
+    finite = y.isfinite()
+    assert torch.equal(got[~finite], y.double()[~finite])
+    error = (got - y.double()).abs() - ref.half_step(dtype) * y.double().abs() - 2.0 ** -22 * size
+    assert (error[finite] <= 0).all()
