@@ -17,7 +17,7 @@ from flux_b200 import operators as ops
 
 class PagedKVCache:
     """Pools of ``pages`` pages of ``page_size`` rows for ``layers`` layers, shared by ``sequences`` sequences of at
-    most ``max_rows`` rows.
+    most ``max_rows`` rows, rounded up to whole pages.
 
     A step: :meth:`advance` gives every listed sequence room for its new row and returns the rows' positions; per
     layer, :meth:`write` rotates and stores the packed QKV rows and :meth:`attend` attends over the cache."""
@@ -30,11 +30,16 @@ class PagedKVCache:
             raise ValueError("paged cache pages must be float32, bfloat16 or float16")
         if head_dim % 8 != 0 or head_dim > 256:
             raise ValueError("paged cache head_dim must be a multiple of 8 up to 256")
+        columns = -(-max_rows // page_size)
+        if (pages > 2 ** 20 or sequences > 2 ** 18 or kv_heads > 65535 or page_size > 65536
+                or columns * page_size >= 2 ** 31):
+            raise ValueError("paged cache sizes must be at most 1048576 pages, 262144 sequences, 65535 KV heads, 65536 "
+                             "rows of a page and 2147483647 rows of a sequence")
         shape = (layers, pages, kv_heads, page_size, head_dim)
         self.page_size = page_size
         self.key_pages = torch.zeros(shape, dtype=dtype, device=device)
         self.value_pages = torch.zeros(shape, dtype=dtype, device=device)
-        self.page_table = torch.full((sequences, -(-max_rows // page_size)), -1, dtype=torch.int32, device=device)
+        self.page_table = torch.full((sequences, columns), -1, dtype=torch.int32, device=device)
         self.lengths = torch.zeros(sequences, dtype=torch.int64, device=device)
         self.page_counts = torch.zeros(pages, dtype=torch.int32, device=device)
 
