@@ -166,8 +166,9 @@ template fx_status launch_paged_merge<__half>(const PagedAttend&, int, cudaStrea
 using namespace fx;
 
 // Query heads of a unit: all that read a KV head, up to 16; of more the largest
-// part that divides them, so that each part reads the rows again (from L2, as a
-// rule: the parts of a KV head are neighbours in the line of tiles).
+// part that divides them, and each part reads the rows again.  64 x 4096 rows of
+// one KV head of 64 BF16 dims take 26 us with 16 query heads, 35 with 32 (two
+// parts) and 45 with 48, but 146 with 17 (17 parts of one head) and 545 with 71.
 static int64_t heads_together(int64_t group) {
     int64_t heads = group < kPagedMaxGroup ? group : kPagedMaxGroup;
     while (group % heads != 0) --heads;

@@ -1,7 +1,7 @@
-// The split of paged decode attention over the GPU, shared by its three kernels:
-// paged_attention_simt.cuh (FP32 pages, up to 4 query heads per KV head),
-// paged_attention_tf32.cuh (FP32 pages, 5-16 heads) and
-// paged_attention_mma.cuh (16-bit pages).
+// The split of paged decode attention over the GPU, shared by its kernels:
+// paged_attention_simt.cu (FP32 pages, up to 4 query heads per KV head),
+// paged_attention_tf32.cu (FP32 pages, 5-16 heads) and paged_attention_mma.cuh
+// (16-bit pages, with queries of their type or FP32 ones).
 //
 // A unit is one (sequence, KV head) with its group of query heads, or one of
 // the equal parts of a group of more than 16; its rows are cut into tiles of kTile rows
@@ -17,8 +17,8 @@
 //
 // Where a unit ends, the warps leave their states in shared memory and all
 // threads join them.  (Going on at once, with one warp that joins for all, was
-// no faster when tried: 51.1 us for 50.8 with 64 sequences of 512-4096 rows, and 2 us
-// slower for a single short one.)  A unit that lies in one CTA is finished
+// no faster in an earlier form of these kernels, and 2 us slower for a single
+// short sequence.)  A unit that lies in one CTA is finished
 // there.  One that spans CTAs leaves (max, sum, unnormalised output) of each
 // piece in the workspace for the merge kernel.  All in an order fixed by the
 // lengths: results repeat bit for bit.
@@ -290,8 +290,10 @@ struct PagedRing {
         }
     }
 
-    // Rows are read once: they are the first to leave L2 (64 sequences of 512-4096
-    // FP32 rows, twelve caches in turn: 46.4 us without the hint, 44.9 with it).
+    // The first to leave L2, since as a rule nobody reads a row again soon (64
+    // sequences of 512-4096 FP32 rows, twelve caches in turn: 46.4 us without the
+    // hint, 44.9 with it).  Parts of a group of more than 16 heads and sequences that
+    // share pages do; what the hint costs them has not been measured.
     static __device__ __forceinline__ void copy16(uint32_t dst, const P* src, uint32_t bytes) {
         uint64_t streamed;
         asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(streamed));

@@ -1,10 +1,12 @@
 // Paged decode attention for FP32 queries on FP32 pages with 5 to 16 query heads
 // per KV head, on the warp-level tensor instructions (m16n8k8, TF32 operands,
 // FP32 accumulators).  The FP32 units would be the bound there: here 8 heads take
-// 53 us and 16 heads 67 for 64 x 4096 rows of 2 KV heads of 64 dims (268 MB, 77 %
-// and 61 % of the measured copy rate; one CTA per SM instead of two: 57 and 77).
-// The products bound it; with 3 heads it is slower than the FP32 units (61 us for
-// 64 x 512-4096 rows when those took 46).
+// 55 us and 16 heads 69 for 64 x 4096 rows of 2 KV heads of 64 dims (268 MB, 74 %
+// and 60 % of the measured copy rate; one CTA per SM instead of two took 57 and 77
+// when two took 53 and 67).  No one unit is full with 16 heads: tensor pipe 37 %,
+// issue slots 58 %, HBM 46 %; warps wait for the products and the splitting before
+// them (math pipe and fixed latency are the first stalls).  With 3 heads it is
+// slower than the FP32 units (61 us for 64 x 512-4096 rows when those took 46).
 //
 // Every operand x is carried as hi = tf32(x) and lo = tf32(x - hi), and a
 // product is hi hi + lo hi + hi lo: what is dropped is below 2^-20 of it.  The
@@ -12,8 +14,8 @@
 // dims share an accumulator and P V is added to the output with an FP32
 // instruction; the cross terms, 2^-11 of the result, have one of their own.  Up to
 // 8 heads leave half of the first operand's rows free: lo lies there, and two
-// products do the work of three (65 -> 52 us for 32 x 2048 rows of 4 KV heads with
-// 8 query heads of 128 dims).
+// products do the work of three (32 x 2048 rows of 4 KV heads with 8 query heads of
+// 128 dims: 65 us -> 52 when that came, 53 now).
 //
 // One warp takes 8 keys at a time:
 //   S [16 heads x 8 keys] = Q K^T, D / 8 steps;
