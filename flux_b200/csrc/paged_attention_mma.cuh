@@ -198,9 +198,9 @@ __global__ void __launch_bounds__(MmaShape<T, Q, DP, Heads>::kThreads, MmaShape<
                         top = fmaxf(top, fmaxf(fabsf(element(i, r, across, 0)), fabsf(element(i, r, across, 1))));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // 2^(13 - floor(log2 top)); 1 where that is no normal number
+                // 2^(13 - floor(log2 top)), or the largest power of two
                 const int bits = 13 + 127 - static_cast<int>((__float_as_uint(top) >> 23) & 255u) + 127;
-                factor[r] = __uint_as_float(bits > 0 && bits < 255 ? static_cast<uint32_t>(bits) << 23 : 127u << 23);
+                factor[r] = __uint_as_float(static_cast<uint32_t>(min(bits, 254)) << 23);
                 scale[r] = a.scale / factor[r];
             }
         }

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from tests import paged_reference as ref
-from tests.test_gpu_paged import _assert_attention, _ops, _randn
+from tests.test_gpu_paged import _assert_attention, _attend_case, _ops, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -86,6 +86,19 @@ def test_attention_with_the_largest_queries_on_16_bit_pages(group):
     out = _ops().paged_gqa_decode_attention_native(q.cuda(), k.cuda(), v.cuda(), table.cuda(), lengths.cuda(), 0.25)
     _assert_attention(out, q, k, v, table, lengths, 0.25)
 
+
+
+@pytest.mark.parametrize("group", [3, 8, 12])
+@pytest.mark.parametrize("size", [1e-34, 1e-35, 1e-37, 1e30, 1e36])
+def test_attention_with_tiny_and_huge_queries_on_float16_pages(group, size):
+    """Float32 queries down to the smallest normal ones, with a scale that makes up for it."""
+    case = _attend_case([300, 5], 16, 2, group, 64, "f32", "f16", seed=5, scale=0.125 / size)
+    q, k, v, kc, vc, table, lengths, scale = case
+    q *= size
+    out = _ops().paged_gqa_decode_attention_native(q.cuda(), kc, vc, table.cuda(), lengths.cuda(), scale)
+    _assert_attention(out, q, k, v, table, lengths, scale)
+    zero = _ops().paged_gqa_decode_attention_native(0 * q.cuda(), kc, vc, table.cuda(), lengths.cuda(), scale)
+    _assert_attention(zero, 0 * q, k, v, table, lengths, scale)
 
 @pytest.mark.parametrize("dim,group", [(64, 4), (128, 8), (256, 3), (64, 16), (128, 9)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
